@@ -48,20 +48,23 @@ class Nb1dBlockStruct(C.Structure):
 DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
+TRANSLATION_UNITS = ("erfnet_hip.hip", "train_ops.hip")
+
+
 def sources():
     return [os.path.join(_SRC, f) for f in sorted(os.listdir(_SRC))] + \
         [os.path.join(os.path.dirname(_HERE), "include", "erfnet_hip.h")]
 
 
 def build(force=False, verbose=False):
-    """Compile csrc/erfnet_hip.hip -> liberfnet_hip.so for gfx950 if it is missing or stale."""
+    """Compile csrc/*.hip -> liberfnet_hip.so for gfx950 if it is missing or stale."""
     srcs = sources()
     if not force and os.path.exists(_SO) and \
             os.path.getmtime(_SO) >= max(os.path.getmtime(s) for s in srcs):
         return _SO
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", *DEVICE_FLAGS,
-           "-o", _SO, os.path.join(_SRC, "erfnet_hip.hip")]
+           "-o", _SO, *(os.path.join(_SRC, f) for f in TRANSLATION_UNITS)]
     if verbose:
         print(" ".join(cmd))
     subprocess.check_call(cmd)
@@ -140,13 +143,24 @@ _PROTOS = {
                                 C.c_double, ll, vp]),
     "erf_sgd_step": (C.c_int, [C.c_int, vp, vp, vp, vp, C.c_double, C.c_double, C.c_double, vp]),
     "erf_ema_update": (C.c_int, [C.c_int, vp, vp, vp, C.c_double, vp]),
+    "erf_layer_norm_workspace_bytes": (C.c_size_t, [ll, C.c_int]),
+    "erf_layer_norm_forward": (C.c_int, [vp, vp, vp, vp, vp, vp, ll, C.c_int, C.c_float, vp]),
+    "erf_layer_norm_backward": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, ll, C.c_int, vp, C.c_size_t, vp]),
+    "erf_log_probs_workspace_bytes": (C.c_size_t, [ll, C.c_int, ll, C.c_int]),
+    "erf_log_probs_forward": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, ll, C.c_int, ll, ll, C.c_int, ll, vp, C.c_size_t, vp]),
+    "erf_log_probs_backward": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, ll, C.c_int, ll, ll, C.c_int, ll, vp]),
+    "erf_adamw_step": (C.c_int, [C.c_int, vp, vp, vp, vp, vp, C.c_double, C.c_double, C.c_double, C.c_double,
+                                 C.c_double, ll, vp]),
+    "erf_adamw8_step": (C.c_int, [C.c_int, vp, vp, vp, vp, vp, vp, vp, C.c_double, C.c_double, C.c_double, C.c_double,
+                                  C.c_double, ll, vp]),
 }
 
 # bf16 variants: same argument lists (activation pointers are bf16 tensors, parameters stay fp32)
 for _n in ("erf_downsampler_forward", "erf_downsampler_backward", "erf_nb1d_forward", "erf_nb1d_chain_forward",
            "erf_nb1d_backward", "erf_nb1d_backward_bits", "erf_upsampler_forward", "erf_upsampler_backward", "erf_outconv_argmax",
            "erf_outconv_backward", "erf_outconv_ce_backward", "erf_outconv_ce_forward", "erf_conv2d_forward", "erf_conv2d_backward", "erf_conv_pair_pack",
-           "erf_conv_pair_forward"):
+           "erf_conv_pair_forward", "erf_layer_norm_forward", "erf_layer_norm_backward", "erf_log_probs_forward",
+           "erf_log_probs_backward", "erf_adamw_step", "erf_adamw8_step"):
     _PROTOS[_n + "_bf16"] = _PROTOS[_n]
 # erf_outconv_forward_bf16 has one more argument: y_is_bf16 behind y
 _PROTOS["erf_outconv_forward_bf16"] = (C.c_int, [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
@@ -157,7 +171,7 @@ OPT_PAIR_FUSION, OPT_WGRAD_LINE, OPT_STREAM16, OPT_PAIR16, OPT_LINE2, OPT_SPLIT_
 OPT_POOL_FUSE = 9
 
 EXPORTS = tuple(_PROTOS)
-ABI_VERSION = 105                         # ERF_ABI_VERSION of include/erfnet_hip.h
+ABI_VERSION = 106                         # ERF_ABI_VERSION of include/erfnet_hip.h
 
 
 def lib():

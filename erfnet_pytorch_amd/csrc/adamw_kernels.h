@@ -1,0 +1,179 @@
+// AdamW (decoupled weight decay) over many tensors at once:
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p = p (1 - lr wd) - (lr / c1) m / (sqrt(v) / sqrt(c2) + eps),
+//   c1 = 1 - b1^t, c2 = 1 - b2^t.
+// Parameters and gradients fp32 or bf16 (widened, rounded once on the way back), arithmetic fp32.
+//
+// BITS = 32 holds m and v in fp32.  BITS = 8 holds m and r = sqrt(v) as float8 (e4m3: 4 significant bits, largest 448) with
+// one fp32 scale, the block's largest magnitude / 448, for each 256 consecutive elements of a tensor.  The root halves v's
+// range in the exponent, so the 2^17 that e4m3 spans cover 2^35 of v, and it is what the denominator needs.  A root
+// that is not zero is never stored as zero: an element whose moment outlives its rounded-off denominator would
+// otherwise move by lr m / eps.  The scale is the largest magnitude itself, not a power of two above it: v
+// moves by 1 - b2 a step, far below half a code, and only through the scale do the codes follow such small moves.
+// NaN and infinity are stored as NaN in their own element and left out of the block's scale.
+//
+// Bound by memory: 28 / 22 bytes an element (fp32 / bf16 parameters) with 32-bit moments, 16 / 10 with 8-bit ones.
+// A wave takes 256 consecutive elements at a time, four a lane: one 16-byte access of fp32, and exactly one scale.
+#pragma once
+#include "vec16.h"
+
+#define ADAMW_MAX_TENSORS 56
+#define ADAMW_BLOCK 256
+#define ADAMW_SCALE_BLOCK 256
+#define ADAMW_ROUNDS 4
+#define ADAMW_CHUNK (ADAMW_BLOCK * 4 * ADAMW_ROUNDS)
+#define ADAMW_TINY 7.8886090522101181e-31f      // 2^-100: 448 / x stays finite above it; blocks below are stored as zeros
+
+struct AdamwDesc {
+    void *p[ADAMW_MAX_TENSORS];
+    const void *g[ADAMW_MAX_TENSORS];
+    void *m[ADAMW_MAX_TENSORS], *v[ADAMW_MAX_TENSORS];          // BITS = 8: codes of m and of r
+    float *ms[ADAMW_MAX_TENSORS], *rs[ADAMW_MAX_TENSORS];       // BITS = 8: scales
+    long long n[ADAMW_MAX_TENSORS];
+    unsigned end_chunk[ADAMW_MAX_TENSORS];      // running total of chunks up to and including tensor i
+    int count;
+    float b1, ob1, b2, ob2, keep, step, root_c2, eps;           // ob = 1 - b, keep = 1 - lr wd, step = lr / c1
+};
+
+__device__ __forceinline__ float adamw_update(const AdamwDesc &d, float p, float g, float &m, float &v, float &root)
+{
+    m = d.b1 * m + d.ob1 * g;
+    v = d.b2 * v + d.ob2 * (g * g);
+    root = sqrtf(v);
+    return p * d.keep - d.step * m / (root / d.root_c2 + d.eps);
+}
+
+// four consecutive elements, the first `left` of them there
+template <typename T> struct AdamwQuad;
+template <> struct AdamwQuad<float> {
+    struct __attribute__((packed, aligned(4))) Raw { f32x4 v; };
+    static __device__ __forceinline__ f32x4 load(const void *p, long long i, int left)
+    {
+        f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float *q = (const float *)p + i;
+        if (left >= 4) r = reinterpret_cast<const Raw *>(q)->v;
+        else
+            for (int j = 0; j < 3; ++j) if (j < left) r[j] = q[j];
+        return r;
+    }
+    static __device__ __forceinline__ void store(void *p, long long i, int left, f32x4 r)
+    {
+        float *q = (float *)p + i;
+        if (left >= 4) reinterpret_cast<Raw *>(q)->v = r;
+        else
+            for (int j = 0; j < 3; ++j) if (j < left) q[j] = r[j];
+    }
+};
+template <> struct AdamwQuad<bf16_t> {
+    struct __attribute__((packed, aligned(2))) Raw { u32x2 v; };
+    static __device__ __forceinline__ f32x4 load(const void *p, long long i, int left)
+    {
+        f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+        const bf16_t *q = (const bf16_t *)p + i;
+        if (left >= 4) r = unpack_bf16x4(reinterpret_cast<const Raw *>(q)->v);
+        else
+            for (int j = 0; j < 3; ++j) if (j < left) r[j] = bf16_to_f32(q[j]);
+        return r;
+    }
+    static __device__ __forceinline__ void store(void *p, long long i, int left, f32x4 r)
+    {
+        bf16_t *q = (bf16_t *)p + i;
+        if (left >= 4) reinterpret_cast<Raw *>(q)->v = pack_bf16x4(r);
+        else
+            for (int j = 0; j < 3; ++j) if (j < left) q[j] = f32_to_bf16(r[j]);
+    }
+};
+struct AdamwCodes {
+    struct __attribute__((packed, aligned(1))) Raw { unsigned v; };
+    static __device__ __forceinline__ unsigned load(const void *p, long long i, int left)
+    {
+        const unsigned char *q = (const unsigned char *)p + i;
+        unsigned r = 0;
+        if (left >= 4) r = reinterpret_cast<const Raw *>(q)->v;
+        else
+            for (int j = 0; j < 3; ++j) if (j < left) r |= (unsigned)q[j] << (8 * j);
+        return r;
+    }
+    static __device__ __forceinline__ void store(void *p, long long i, int left, unsigned r)
+    {
+        unsigned char *q = (unsigned char *)p + i;
+        if (left >= 4) reinterpret_cast<Raw *>(q)->v = r;
+        else
+            for (int j = 0; j < 3; ++j) if (j < left) q[j] = (unsigned char)(r >> (8 * j));
+    }
+    static __device__ __forceinline__ f32x4 decode(unsigned r, float scale)
+    {
+        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)r, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)r, true);
+        return (f32x4){a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale};
+    }
+    // codes of x at the wave's own scale (all 64 lanes take part); ROOT: x >= 0 and nonzero stays nonzero
+    template <bool ROOT> static __device__ __forceinline__ unsigned encode(f32x4 x, float &scale)
+    {
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float a = fabsf(x[j]);
+            top = fmaxf(top, a < INFINITY ? a : 0.0f);
+        }
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const bool some = top >= ADAMW_TINY;
+        const float inv = some ? 448.0f / top : 0.0f;
+        scale = some ? top / 448.0f : 0.0f;
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            y[j] = x[j] * inv;
+            if (ROOT && some && x[j] > 0.0f) y[j] = fmaxf(y[j], 0.001953125f);     // 2^-9, the least code above zero
+            if (!(fabsf(x[j]) < INFINITY)) y[j] = __builtin_nanf("");
+        }
+        int r = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], r, true);
+        return (unsigned)r;
+    }
+};
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(ADAMW_BLOCK) void adamw_kernel(const AdamwDesc d)
+{
+    // the tensor of this chunk: the number of running totals that are not above it (64 lanes look at all of them)
+    const int lane = threadIdx.x & 63;
+    const bool past = lane < d.count && blockIdx.x >= d.end_chunk[lane < d.count ? lane : 0];
+    const int t = __popcll(__ballot(past));
+    const unsigned first = t ? d.end_chunk[t - 1] : 0u;
+    const long long n = d.n[t];
+    const long long base = (long long)(blockIdx.x - first) * ADAMW_CHUNK + (threadIdx.x >> 6) * ADAMW_SCALE_BLOCK;
+#pragma unroll
+    for (int r = 0; r < ADAMW_ROUNDS; ++r) {
+        const long long at = base + (long long)r * ADAMW_BLOCK * 4;       // this wave's 256 elements
+        if (at >= n) break;                                             // (uniform over the wave)
+        const long long i = at + lane * 4;
+        const int left = n - i >= 4 ? 4 : (int)(n - i);                 // may be negative
+        f32x4 p = AdamwQuad<T>::load(d.p[t], i, left);
+        const f32x4 g = AdamwQuad<T>::load(d.g[t], i, left);
+        f32x4 m, v, root;
+        if (BITS == 32) {
+            m = AdamwQuad<float>::load(d.m[t], i, left);
+            v = AdamwQuad<float>::load(d.v[t], i, left);
+        } else {
+            m = AdamwCodes::decode(AdamwCodes::load(d.m[t], i, left), d.ms[t][at / ADAMW_SCALE_BLOCK]);
+            v = AdamwCodes::decode(AdamwCodes::load(d.v[t], i, left), d.rs[t][at / ADAMW_SCALE_BLOCK]);
+            v *= v;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float mj = m[j], vj = v[j], rj;
+            p[j] = adamw_update(d, p[j], g[j], mj, vj, rj);
+            m[j] = mj; v[j] = vj; root[j] = rj;
+        }
+        AdamwQuad<T>::store(d.p[t], i, left, p);
+        if (BITS == 32) {
+            AdamwQuad<float>::store(d.m[t], i, left, m);
+            AdamwQuad<float>::store(d.v[t], i, left, v);
+        } else {
+            float ms, rs;
+            const unsigned cm = AdamwCodes::encode<false>(m, ms), cr = AdamwCodes::encode<true>(root, rs);
+            AdamwCodes::store(d.m[t], i, left, cm);
+            AdamwCodes::store(d.v[t], i, left, cr);
+            if (lane == 0) { d.ms[t][at / ADAMW_SCALE_BLOCK] = ms; d.rs[t][at / ADAMW_SCALE_BLOCK] = rs; }
+        }
+    }
+}

@@ -18,6 +18,7 @@
 #include "loss_kernels.h"
 #include "metric_kernels.h"
 #include "optim_kernels.h"
+#include "host.h"
 
 #include <algorithm>
 #include <atomic>
@@ -1730,6 +1731,21 @@ int opt_launch(const char *what, int count, float *const *p, const float *const 
     return 0;
 }
 }  // namespace
+
+int host_fail(const char *fmt, ...)
+{
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return 1;
+}
+
+int host_launched(const char *kernel)
+{
+    CHECK_LAUNCH(kernel);
+    return 0;
+}
 
 extern "C" {
 

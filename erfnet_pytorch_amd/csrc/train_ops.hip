@@ -1,0 +1,406 @@
+// liberfnet_hip.so — C ABI (include/erfnet_hip.h) over norm_kernels.h, logprob_kernels.h and adamw_kernels.h: layer norm,
+// token log probabilities, AdamW.  A translation unit of its own; as in erfnet_hip.hip the host side builds descriptors and
+// launches, and never allocates, copies or synchronises.
+#include "../../include/erfnet_hip.h"
+#include "host.h"
+#include "adamw_kernels.h"
+#include "logprob_kernels.h"
+#include "norm_kernels.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+namespace {
+
+#define fail host_fail
+#define LAUNCHED(name)                                                                             \
+    do {                                                                                           \
+        if (host_launched(name)) return 1;                                                         \
+    } while (0)
+
+int log2_up(int v)
+{
+    int b = 0;
+    while ((1 << b) < v) ++b;
+    return b;
+}
+
+// ================================================================================ layer norm
+// A row of up to 16 elements a lane and 64 lanes stays inside a wave (no barrier, several short rows a wave);
+// longer rows take a block, one to four vectors a thread.
+struct NormPlan {
+    bool wave;
+    int rounds, lanes, threads;
+};
+template <typename T> NormPlan norm_plan(int C)
+{
+    const int vecs = (C + Vec16<T>::N - 1) / Vec16<T>::N, most = 16 / Vec16<T>::N;
+    NormPlan p = {true, 1, 64, NORM_BLOCK};
+    if (vecs <= 64 * most) {
+        while (p.rounds * 64 < vecs) p.rounds *= 2;
+        p.lanes = 1 << log2_up((vecs + p.rounds - 1) / p.rounds);
+        return p;
+    }
+    p.wave = false;
+    while (p.rounds * 1024 < vecs) p.rounds *= 2;
+    p.threads = ((vecs + p.rounds - 1) / p.rounds + 63) / 64 * 64;
+    return p;
+}
+int norm_blocks(const NormPlan &p, long long rows, int most)
+{
+    const long long per = p.wave ? NORM_BLOCK / p.lanes : 1;
+    return (int)std::min<long long>((rows + per - 1) / per, most);
+}
+#define NORM_BWD_BLOCKS(p) ((p).wave ? 1024 : (p).threads > 512 ? 256 : 512)
+
+int norm_check(const char *what, const void *x, const void *y, long long rows, int C, float eps)
+{
+    if (rows < 0) return fail("%s: negative row count", what);
+    if (C < 1 || C > NORM_MAX_C) return fail("%s: 1..%d channels (got %d)", what, NORM_MAX_C, C);
+    if (!(eps >= 0.0f)) return fail("%s: eps must not be negative", what);
+    if (rows && (!x || !y)) return fail("%s: null pointer", what);
+    return 0;
+}
+
+template <typename T>
+int norm_forward(const void *x, const float *w, const float *b, void *y, float *mean, float *rstd, long long rows, int C,
+                 float eps, hipStream_t st)
+{
+    if (norm_check("layer norm", x, y, rows, C, eps)) return 1;
+    if (!mean != !rstd) return fail("layer norm: mean and rstd are kept together");
+    if (rows == 0) return 0;
+    const NormPlan p = norm_plan<T>(C);
+    NormDesc d;
+    memset(&d, 0, sizeof(d));
+    d.x = x; d.y = y; d.w = w; d.b = b; d.mean = mean; d.rstd = rstd;
+    d.rows = rows; d.C = C; d.eps = eps; d.lanes = p.lanes; d.lane_bits = log2_up(p.lanes);
+    const int blocks = norm_blocks(p, rows, 2048);
+    if (p.wave) {
+        if (p.rounds == 1) norm_fwd_wave_kernel<T, 1><<<blocks, NORM_BLOCK, 0, st>>>(d);
+        else if (p.rounds == 2) norm_fwd_wave_kernel<T, 2><<<blocks, NORM_BLOCK, 0, st>>>(d);
+        else if constexpr (Vec16<T>::N == 4) norm_fwd_wave_kernel<T, 4><<<blocks, NORM_BLOCK, 0, st>>>(d);
+        LAUNCHED("norm_fwd_wave_kernel");
+        return 0;
+    }
+    if (p.rounds == 1) norm_fwd_block_kernel<T, 1><<<blocks, p.threads, 0, st>>>(d);
+    else if (p.rounds == 2) norm_fwd_block_kernel<T, 2><<<blocks, p.threads, 0, st>>>(d);
+    else if constexpr (Vec16<T>::N == 4) norm_fwd_block_kernel<T, 4><<<blocks, p.threads, 0, st>>>(d);
+    LAUNCHED("norm_fwd_block_kernel");
+    return 0;
+}
+
+template <typename T> size_t norm_ws(long long rows, int C)
+{
+    const NormPlan p = norm_plan<T>(C);
+    return (size_t)norm_blocks(p, rows, NORM_BWD_BLOCKS(p)) * 2 * C * sizeof(float);
+}
+
+template <typename T>
+int norm_backward(const void *x, const float *w, const float *mean, const float *rstd, const void *gy, void *dx, float *dw,
+                  float *db, long long rows, int C, void *ws, size_t ws_bytes, hipStream_t st)
+{
+    if (norm_check("layer norm backward", x, gy, rows, C, 0.0f)) return 1;
+    const bool params = dw || db;
+    if (rows && (!mean || !rstd)) return fail("layer norm backward: null pointer");
+    if (!dx && !params) return 0;
+    const NormPlan p = norm_plan<T>(C);
+    const int blocks = norm_blocks(p, rows, NORM_BWD_BLOCKS(p));
+    NormDesc d;
+    memset(&d, 0, sizeof(d));
+    d.x = x; d.gy = gy; d.y = dx; d.w = w; d.mean = const_cast<float *>(mean); d.rstd = const_cast<float *>(rstd);
+    d.rows = rows; d.C = C; d.lanes = p.lanes; d.lane_bits = log2_up(p.lanes);
+    if (params) {
+        if (blocks && (!ws || ws_bytes < norm_ws<T>(rows, C))) return fail("layer norm backward: workspace too small");
+        d.partial = (float *)ws;
+    }
+    if (blocks) {
+        if (p.wave) {
+            const size_t lds = params ? (size_t)8 * C * sizeof(float) : 0;
+            if (p.rounds == 1) norm_bwd_wave_kernel<T, 1><<<blocks, NORM_BLOCK, lds, st>>>(d);
+            else if (p.rounds == 2) norm_bwd_wave_kernel<T, 2><<<blocks, NORM_BLOCK, lds, st>>>(d);
+            else if constexpr (Vec16<T>::N == 4) norm_bwd_wave_kernel<T, 4><<<blocks, NORM_BLOCK, lds, st>>>(d);
+            LAUNCHED("norm_bwd_wave_kernel");
+        } else {
+            if (p.rounds == 1) norm_bwd_block_kernel<T, 1><<<blocks, p.threads, 0, st>>>(d);
+            else if (p.rounds == 2) norm_bwd_block_kernel<T, 2><<<blocks, p.threads, 0, st>>>(d);
+            else if constexpr (Vec16<T>::N == 4) norm_bwd_block_kernel<T, 4><<<blocks, p.threads, 0, st>>>(d);
+            LAUNCHED("norm_bwd_block_kernel");
+        }
+    }
+    if (params) {
+        norm_grad_sum_kernel<<<(2 * C + 31) / 32, 1024, 0, st>>>((const float *)ws, blocks, C, dw, db);   // (no rows: zeros)
+        LAUNCHED("norm_grad_sum_kernel");
+    }
+    return 0;
+}
+
+// ================================================================================ token log probabilities
+#define LP_MAX_CLASSES (1 << 30)
+
+// Blocks per row: a wave takes a row of up to 2048 classes; longer ones take whole blocks, several when the rows alone
+// would leave compute units without work (about four blocks each), with at least 2048 classes in every block.
+struct LpPlan {
+    bool wave;
+    int splits, seg;
+};
+LpPlan lp_plan(long long rows, int V)
+{
+    LpPlan p = {V <= 2048, 1, V};
+    if (p.wave) return p;
+    const long long want = (1024 + rows - 1) / std::max<long long>(rows, 1);
+    p.splits = (int)std::min<long long>(std::max<long long>(want, 1), (V + 2047) / 2048);
+    p.seg = ((V + p.splits - 1) / p.splits + 2047) / 2048 * 2048;
+    p.splits = (V + p.seg - 1) / p.seg;
+    return p;
+}
+size_t lp_ws(long long outer, int V, long long inner, int k)
+{
+    if (inner > 1) return 0;
+    const LpPlan p = lp_plan(outer, V);
+    return p.splits > 1 ? (size_t)outer * p.splits * (sizeof(float4) + (size_t)k * 8) : 0;
+}
+
+int lp_check(const char *what, long long outer, int V, long long inner, int k)
+{
+    if (outer < 0 || inner < 1) return fail("%s: negative or empty extent", what);
+    if (V < 1 || V > LP_MAX_CLASSES) return fail("%s: 1..%d classes (got %d)", what, LP_MAX_CLASSES, V);
+    const int most = inner > 1 ? ERF_LOG_PROBS_MAX_TOP_PIXELS : ERF_LOG_PROBS_MAX_TOP;
+    if (k < 0 || k > most || k > V) return fail("%s: top_k must be in 0..%d and at most the class count (got %d)", what, most, k);
+    // one block per 256 pixels or per (row, segment): the grid must fit 31 bits
+    if (outer > (1ll << 40) / inner) return fail("%s: too many rows", what);
+    const long long blocks = inner > 1 ? (outer * inner + LP_BLOCK - 1) / LP_BLOCK
+                                       : V <= 2048 ? (outer + 3) / 4 : outer * ((V + 8191) / 8192);
+    if (blocks >= (1ll << 31)) return fail("%s: too many rows", what);
+    return 0;
+}
+
+template <typename T>
+int lp_forward(const void *x, const long long *target, float *log_prob, float *entropy, float *stats, float *top_lp,
+               long long *top_idx, long long outer, int V, long long inner, long long ld, int k, long long ignore, void *ws,
+               size_t ws_bytes, hipStream_t st)
+{
+    if (lp_check("log_probs", outer, V, inner, k)) return 1;
+    if (outer == 0) return 0;
+    if (!x || !target || !log_prob || !entropy || !stats || (k && (!top_lp || !top_idx))) return fail("log_probs: null pointer");
+    if (inner == 1 && ld < V && outer > 1) return fail("log_probs: rows overlap (stride %lld, %d classes)", ld, V);
+    LpDesc d;
+    memset(&d, 0, sizeof(d));
+    d.x = x; d.target = target; d.log_prob = log_prob; d.entropy = entropy; d.stats = (float2 *)stats;
+    d.top_lp = top_lp; d.top_idx = top_idx; d.rows = outer * inner; d.ld = ld; d.inner = inner; d.ignore = ignore;
+    d.V = V; d.k = k;
+    if (inner > 1) {
+        const unsigned blocks = (unsigned)((d.rows + LP_BLOCK - 1) / LP_BLOCK);
+        if (k == 0) lp_pixels_kernel<T, 0><<<blocks, LP_BLOCK, 0, st>>>(d);
+        else if (k == 1) lp_pixels_kernel<T, 1><<<blocks, LP_BLOCK, 0, st>>>(d);
+        else if (k == 2) lp_pixels_kernel<T, 2><<<blocks, LP_BLOCK, 0, st>>>(d);
+        else if (k <= 4) lp_pixels_kernel<T, 4><<<blocks, LP_BLOCK, 0, st>>>(d);
+        else lp_pixels_kernel<T, 8><<<blocks, LP_BLOCK, 0, st>>>(d);
+        LAUNCHED("lp_pixels_kernel");
+        return 0;
+    }
+    const LpPlan p = lp_plan(outer, V);
+    d.splits = p.splits; d.seg = p.seg;
+    if (p.splits > 1) {
+        if (!ws || ws_bytes < lp_ws(outer, V, inner, k)) return fail("log_probs: workspace too small");
+        d.part = (float4 *)ws;
+        d.part_keys = (unsigned long long *)((char *)ws + (size_t)outer * p.splits * sizeof(float4));
+    }
+    if (p.wave) {
+        const unsigned blocks = (unsigned)((outer + 3) / 4);
+        if (k) lp_rows_kernel<T, 64, true><<<blocks, LP_BLOCK, 0, st>>>(d);
+        else lp_rows_kernel<T, 64, false><<<blocks, LP_BLOCK, 0, st>>>(d);
+    } else {
+        const unsigned blocks = (unsigned)(outer * p.splits);
+        if (k) lp_rows_kernel<T, 256, true><<<blocks, LP_BLOCK, 0, st>>>(d);
+        else lp_rows_kernel<T, 256, false><<<blocks, LP_BLOCK, 0, st>>>(d);
+    }
+    LAUNCHED("lp_rows_kernel");
+    if (p.splits > 1) {
+        lp_join_kernel<T><<<(unsigned)outer, LP_BLOCK, 0, st>>>(d);
+        LAUNCHED("lp_join_kernel");
+    }
+    return 0;
+}
+
+template <typename T>
+int lp_backward(const void *x, const long long *target, const float *entropy, const float *stats, const long long *top_idx,
+                const float *g_lp, const float *g_h, const float *g_top, void *dx, long long outer, int V, long long inner,
+                long long ld, int k, long long ignore, hipStream_t st)
+{
+    if (lp_check("log_probs backward", outer, V, inner, k)) return 1;
+    if (outer == 0) return 0;
+    if (!x || !target || !entropy || !stats || !dx || (k && !top_idx)) return fail("log_probs backward: null pointer");
+    LpDesc d;
+    memset(&d, 0, sizeof(d));
+    d.x = x; d.target = target; d.entropy = const_cast<float *>(entropy); d.stats = (float2 *)const_cast<float *>(stats);
+    d.top_idx = const_cast<long long *>(top_idx); d.g_lp = g_lp; d.g_h = g_h; d.g_top = g_top; d.dx = dx;
+    d.rows = outer * inner; d.ld = ld; d.inner = inner; d.ignore = ignore; d.V = V; d.k = k;
+    if (inner > 1) {
+        const unsigned blocks = (unsigned)((d.rows + LP_BLOCK - 1) / LP_BLOCK);
+        if (!g_top || k == 0) lp_pixels_bwd_kernel<T, 0><<<blocks, LP_BLOCK, 0, st>>>(d);
+        else if (k <= 2) lp_pixels_bwd_kernel<T, 2><<<blocks, LP_BLOCK, 0, st>>>(d);
+        else lp_pixels_bwd_kernel<T, 8><<<blocks, LP_BLOCK, 0, st>>>(d);
+        LAUNCHED("lp_pixels_bwd_kernel");
+        return 0;
+    }
+    if (V <= 2048) {
+        lp_rows_bwd_kernel<T, 64><<<(unsigned)((outer + 3) / 4), LP_BLOCK, 0, st>>>(d);
+    } else {
+        d.seg = 8192;
+        d.splits = (V + d.seg - 1) / d.seg;
+        lp_rows_bwd_kernel<T, 256><<<(unsigned)(outer * d.splits), LP_BLOCK, 0, st>>>(d);
+    }
+    LAUNCHED("lp_rows_bwd_kernel");
+    return 0;
+}
+
+// ================================================================================ AdamW
+template <typename T, int BITS>
+int adamw_step(const char *what, int count, void *const *p, const void *const *g, void *const *m, float *const *ms,
+               void *const *v, float *const *vs, const long long *numel, double lr, double b1, double b2, double eps,
+               double wd, long long step, hipStream_t st)
+{
+    if (count < 0) return fail("%s: negative tensor count", what);
+    if (step < 1) return fail("%s: step counts from 1 (got %lld)", what, step);
+    if (!(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0)) return fail("%s: betas outside [0, 1)", what);
+    if (!(eps >= 0.0) || !(lr >= 0.0) || !(wd >= 0.0)) return fail("%s: negative lr / eps / weight decay", what);
+    if (count && (!p || !g || !m || !v || !numel || (BITS == 8 && (!ms || !vs)))) return fail("%s: null pointer table", what);
+    AdamwDesc d;
+    memset(&d, 0, sizeof(d));
+    // the scalars in double, rounded once for the kernel
+    d.b1 = (float)b1; d.ob1 = (float)(1.0 - b1); d.b2 = (float)b2; d.ob2 = (float)(1.0 - b2);
+    d.keep = (float)(1.0 - lr * wd);
+    d.step = (float)(lr / (1.0 - pow(b1, (double)step)));
+    d.root_c2 = (float)sqrt(1.0 - pow(b2, (double)step));
+    d.eps = (float)eps;
+    for (int i = 0; i < count; ++i) {
+        if (numel[i] < 0) return fail("%s: tensor %d has a negative size", what, i);
+        if (numel[i] && (!p[i] || !g[i] || !m[i] || !v[i] || (BITS == 8 && (!ms[i] || !vs[i]))))
+            return fail("%s: tensor %d has a null pointer", what, i);
+        if (numel[i] / ADAMW_CHUNK >= (1ll << 31) - 1) return fail("%s: tensor %d is too large", what, i);
+    }
+    int i = 0;
+    while (i < count) {
+        d.count = 0;
+        unsigned long long chunks = 0;
+        for (; i < count && d.count < ADAMW_MAX_TENSORS; ++i) {
+            if (numel[i] == 0) continue;
+            const unsigned long long c = ((unsigned long long)numel[i] + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
+            if (chunks + c >= (1ull << 31)) break;              // goes into the next launch
+            const int k = d.count++;
+            d.p[k] = p[i]; d.g[k] = g[i]; d.m[k] = m[i]; d.v[k] = v[i];
+            d.ms[k] = BITS == 8 ? ms[i] : nullptr;
+            d.rs[k] = BITS == 8 ? vs[i] : nullptr;
+            d.n[k] = numel[i];
+            chunks += c;
+            d.end_chunk[k] = (unsigned)chunks;
+        }
+        if (d.count == 0) continue;
+        adamw_kernel<T, BITS><<<(unsigned)chunks, ADAMW_BLOCK, 0, st>>>(d);
+        LAUNCHED("adamw_kernel");
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t erf_layer_norm_workspace_bytes(long long rows, int C)
+{
+    return rows < 0 || C < 1 || C > NORM_MAX_C ? 0 : std::max(norm_ws<float>(rows, C), norm_ws<bf16_t>(rows, C));
+}
+int erf_layer_norm_forward(const float *x, const float *w, const float *b, float *y, float *mean, float *rstd, long long rows,
+                           int C, float eps, void *stream)
+{
+    return norm_forward<float>(x, w, b, y, mean, rstd, rows, C, eps, (hipStream_t)stream);
+}
+int erf_layer_norm_forward_bf16(const void *x, const float *w, const float *b, void *y, float *mean, float *rstd,
+                                long long rows, int C, float eps, void *stream)
+{
+    return norm_forward<bf16_t>(x, w, b, y, mean, rstd, rows, C, eps, (hipStream_t)stream);
+}
+int erf_layer_norm_backward(const float *x, const float *w, const float *mean, const float *rstd, const float *gy, float *dx,
+                            float *dw, float *db, long long rows, int C, void *ws, size_t ws_bytes, void *stream)
+{
+    return norm_backward<float>(x, w, mean, rstd, gy, dx, dw, db, rows, C, ws, ws_bytes, (hipStream_t)stream);
+}
+int erf_layer_norm_backward_bf16(const void *x, const float *w, const float *mean, const float *rstd, const void *gy,
+                                 void *dx, float *dw, float *db, long long rows, int C, void *ws, size_t ws_bytes,
+                                 void *stream)
+{
+    return norm_backward<bf16_t>(x, w, mean, rstd, gy, dx, dw, db, rows, C, ws, ws_bytes, (hipStream_t)stream);
+}
+
+size_t erf_log_probs_workspace_bytes(long long outer, int V, long long inner, int top_k)
+{
+    return outer < 1 || V < 1 || V > LP_MAX_CLASSES || inner < 1 || top_k < 0 || top_k > LP_MAX_TOP
+               ? 0 : lp_ws(outer, V, inner, top_k);
+}
+int erf_log_probs_forward(const float *logits, const long long *target, float *log_prob, float *entropy, float *stats,
+                          float *top_log_probs, long long *top_indices, long long outer, int V, long long inner,
+                          long long row_stride, int top_k, long long ignore_index, void *ws, size_t ws_bytes, void *stream)
+{
+    return lp_forward<float>(logits, target, log_prob, entropy, stats, top_log_probs, top_indices, outer, V, inner, row_stride,
+                             top_k, ignore_index, ws, ws_bytes, (hipStream_t)stream);
+}
+int erf_log_probs_forward_bf16(const void *logits, const long long *target, float *log_prob, float *entropy, float *stats,
+                               float *top_log_probs, long long *top_indices, long long outer, int V, long long inner,
+                               long long row_stride, int top_k, long long ignore_index, void *ws, size_t ws_bytes,
+                               void *stream)
+{
+    return lp_forward<bf16_t>(logits, target, log_prob, entropy, stats, top_log_probs, top_indices, outer, V, inner,
+                              row_stride, top_k, ignore_index, ws, ws_bytes, (hipStream_t)stream);
+}
+int erf_log_probs_backward(const float *logits, const long long *target, const float *entropy, const float *stats,
+                           const long long *top_indices, const float *g_log_prob, const float *g_entropy,
+                           const float *g_top, float *dlogits, long long outer, int V, long long inner,
+                           long long row_stride, int top_k, long long ignore_index, void *stream)
+{
+    return lp_backward<float>(logits, target, entropy, stats, top_indices, g_log_prob, g_entropy, g_top, dlogits, outer, V,
+                              inner, row_stride, top_k, ignore_index, (hipStream_t)stream);
+}
+int erf_log_probs_backward_bf16(const void *logits, const long long *target, const float *entropy, const float *stats,
+                                const long long *top_indices, const float *g_log_prob, const float *g_entropy,
+                                const float *g_top, void *dlogits, long long outer, int V, long long inner,
+                                long long row_stride, int top_k, long long ignore_index, void *stream)
+{
+    return lp_backward<bf16_t>(logits, target, entropy, stats, top_indices, g_log_prob, g_entropy, g_top, dlogits, outer, V,
+                               inner, row_stride, top_k, ignore_index, (hipStream_t)stream);
+}
+
+int erf_adamw_step(int count, float *const *params, const float *const *grads, float *const *exp_avg,
+                   float *const *exp_avg_sq, const long long *numel, double lr, double beta1, double beta2, double eps,
+                   double weight_decay, long long step, void *stream)
+{
+    return adamw_step<float, 32>("adamw", count, (void *const *)params, (const void *const *)grads, (void *const *)exp_avg,
+                                 nullptr, (void *const *)exp_avg_sq, nullptr, numel, lr, beta1, beta2, eps, weight_decay, step,
+                                 (hipStream_t)stream);
+}
+int erf_adamw_step_bf16(int count, void *const *params, const void *const *grads, float *const *exp_avg,
+                        float *const *exp_avg_sq, const long long *numel, double lr, double beta1, double beta2,
+                        double eps, double weight_decay, long long step, void *stream)
+{
+    return adamw_step<bf16_t, 32>("adamw", count, params, grads, (void *const *)exp_avg, nullptr, (void *const *)exp_avg_sq,
+                                  nullptr, numel, lr, beta1, beta2, eps, weight_decay, step, (hipStream_t)stream);
+}
+int erf_adamw8_step(int count, float *const *params, const float *const *grads, void *const *exp_avg,
+                    float *const *exp_avg_scale, void *const *exp_avg_sq_root, float *const *exp_avg_sq_root_scale,
+                    const long long *numel, double lr, double beta1, double beta2, double eps, double weight_decay,
+                    long long step, void *stream)
+{
+    return adamw_step<float, 8>("adamw8", count, (void *const *)params, (const void *const *)grads, exp_avg, exp_avg_scale,
+                                exp_avg_sq_root, exp_avg_sq_root_scale, numel, lr, beta1, beta2, eps, weight_decay, step,
+                                (hipStream_t)stream);
+}
+int erf_adamw8_step_bf16(int count, void *const *params, const void *const *grads, void *const *exp_avg,
+                         float *const *exp_avg_scale, void *const *exp_avg_sq_root, float *const *exp_avg_sq_root_scale,
+                         const long long *numel, double lr, double beta1, double beta2, double eps, double weight_decay,
+                         long long step, void *stream)
+{
+    return adamw_step<bf16_t, 8>("adamw8", count, params, grads, exp_avg, exp_avg_scale, exp_avg_sq_root,
+                                 exp_avg_sq_root_scale, numel, lr, beta1, beta2, eps, weight_decay, step, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,78 @@
+// 16-byte accesses to rows that start at any element (gfx950 global loads and stores take any byte
+// address; the packed types below tell the compiler so).  A row of an odd length keeps the wide access:
+// only the lane that holds the row's last, partial vector goes element by element.
+#pragma once
+#include "common.h"
+
+template <typename T> struct Vec16;
+template <> struct Vec16<float> {
+    static constexpr int N = 4;
+    struct __attribute__((packed, aligned(4))) Raw { u32x4 v; };
+    static __device__ __forceinline__ void unpack(u32x4 r, float (&f)[4])
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned u = r[i];        // (a bit cast of the vector's element itself reads element 0)
+            f[i] = __builtin_bit_cast(float, u);
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[4])
+    {
+        u32x4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(unsigned, f[i]);
+        return r;
+    }
+    static __device__ __forceinline__ float get(const float *p) { return *p; }
+    static __device__ __forceinline__ void put(float *p, float f) { *p = f; }
+};
+template <> struct Vec16<bf16_t> {
+    static constexpr int N = 8;
+    struct __attribute__((packed, aligned(2))) Raw { u32x4 v; };
+    static __device__ __forceinline__ void unpack(u32x4 r, float (&f)[8])
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __builtin_bit_cast(float, r[i] << 16);
+            f[2 * i + 1] = __builtin_bit_cast(float, r[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[8])
+    {
+        u32x4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){f[2 * i], f[2 * i + 1]}, bf16x2));
+        return r;
+    }
+    static __device__ __forceinline__ float get(const bf16_t *p) { return bf16_to_f32(*p); }
+    static __device__ __forceinline__ void put(bf16_t *p, float f) { *p = f32_to_bf16(f); }
+};
+
+// `left` elements of the row begin at p; elements from `left` on read as zero.
+template <typename T> __device__ __forceinline__ u32x4 ld16(const T *p, int left)
+{
+    u32x4 r = {0u, 0u, 0u, 0u};
+    if (left >= Vec16<T>::N) {
+        r = reinterpret_cast<const typename Vec16<T>::Raw *>(p)->v;
+    } else if (left > 0) {
+        constexpr int per = 4 / sizeof(T);      // elements of one 32-bit word
+#pragma unroll
+        for (int i = 0; i < Vec16<T>::N - 1; ++i)
+            if (i < left) {
+                const unsigned bits = sizeof(T) == 4 ? __builtin_bit_cast(unsigned, (float)Vec16<T>::get(p + i))
+                                                     : __builtin_bit_cast(unsigned, (float)Vec16<T>::get(p + i)) >> 16;
+                r[i / per] |= bits << (i % per * 16);
+            }
+    }
+    return r;
+}
+template <typename T> __device__ __forceinline__ void st16(T *p, const float (&f)[Vec16<T>::N], int left)
+{
+    if (left >= Vec16<T>::N) {
+        reinterpret_cast<typename Vec16<T>::Raw *>(p)->v = Vec16<T>::pack(f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Vec16<T>::N - 1; ++i)
+            if (i < left) Vec16<T>::put(p + i, f[i]);
+    }
+}

@@ -7,6 +7,7 @@ transposed convolution NCHW-contiguous so that torch's loss / argmax read them d
 """
 import ctypes as C
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -181,6 +182,9 @@ class _InferenceCtx:
         self.needs_input_grad = (False,) * n_inputs
 
     def save_for_backward(self, *tensors):
+        pass
+
+    def mark_non_differentiable(self, *tensors):
         pass
 
 
@@ -1270,3 +1274,184 @@ class _MseMean(torch.autograd.Function):
 def mse_mean(a, b):
     """mean((a - b)^2) (the elementwise part of MSELossWeighted, train/evaluation_functions.py:122-131)."""
     return _MseMean.apply(a, b)
+
+
+# ------------------------------------------------------------------------------ layer norm
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, eps, axis):
+        # rows of C contiguous channels: the last axis as it is, axis 1 of an image as NHWC memory
+        x = _nhwc(x) if axis == 1 else x.contiguous()
+        c = x.shape[axis]
+        rows = x.numel() // c
+        y = _empty_nhwc(*x.shape, x) if axis == 1 else torch.empty_like(x)
+        kept = any(ctx.needs_input_grad[:3])
+        stat = torch.empty((2, rows), dtype=torch.float32, device=x.device) if kept else None
+        with _dev_ctx(x):
+            _lib.check(_fn("erf_layer_norm_forward", x)(
+                _p(x), _p(_param(w)), _p(_param(b)), _p(y), _p(stat), None if stat is None else vp(stat.data_ptr() + 4 * rows),
+                rows, c, eps, _stream(x)))
+        if kept:
+            ctx.save_for_backward(x, w, stat)
+            ctx.axis, ctx.params = axis, (w, b)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, w, stat = ctx.saved_tensors
+        c, rows = x.shape[ctx.axis], stat.shape[1]
+        if ctx.axis == 1:
+            gy = _nhwc(gy, x.dtype)
+        else:
+            gy = gy.to(x.dtype).contiguous()
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = _empty_nhwc(*x.shape, x) if ctx.axis == 1 else torch.empty_like(x)
+        tg = _grad_targets(ctx.params, [(c,) if need else None for need in ctx.needs_input_grad[1:3]], x.device)
+        ws, n_ws = None, 0
+        if tg[0][0] is not None or tg[1][0] is not None:
+            n_ws = _lib.lib().erf_layer_norm_workspace_bytes(rows, c)
+            ws = torch.empty(n_ws, dtype=torch.uint8, device=x.device)
+        with _dev_ctx(x):
+            _lib.check(_fn("erf_layer_norm_backward", x)(
+                _p(x), _p(_param(w)), _p(stat), vp(stat.data_ptr() + 4 * rows), _p(gy), _p(dx), _p(tg[0][0]), _p(tg[1][0]),
+                rows, c, _p(ws), n_ws, _stream(x)))
+        dw, db = _match_params(_deliver(tg), ctx.params)
+        return dx, dw, db, None, None
+
+
+def _need_gpu(what, x, *others):
+    if not x.is_cuda:
+        raise RuntimeError(f"{what}: the tensor lives on {x.device}; the kernels run on the GPU only")
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise RuntimeError(f"{what}: tensors on {x.device} and {t.device}")
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, dim=-1):
+    """(x - mean) / sqrt(var + eps) * weight + bias over one axis, with its gradients: the last axis, or ``dim=1`` of an
+    [N,C,H,W] activation (every pixel over its channels, which are contiguous in the framework's NHWC memory).  x fp32 or
+    bf16 with 1..16384 channels; weight, bias: [C] or None.  The result has x's type; statistics, products and sums are
+    fp32.  No counterpart in the reference, whose blocks normalise over the batch (train/erfnet_blocks.py:23)."""
+    _check_act(x)
+    nd = x.dim()
+    axis = dim + nd if dim < 0 else dim
+    if not (nd >= 1 and (axis == nd - 1 or (nd == 4 and axis == 1))):
+        raise ValueError(f"layer_norm: dim must be the last axis, or 1 of an [N,C,H,W] tensor (got {dim} for "
+                         f"{tuple(x.shape)})")
+    c = x.shape[axis]
+    for t, what in ((weight, "weight"), (bias, "bias")):
+        if t is not None and tuple(t.shape) != (c,):
+            raise ValueError(f"layer_norm: {what} shape {tuple(t.shape)} does not match {c} channels")
+    if not 1 <= c <= 16384:
+        raise ValueError(f"layer_norm: 1..16384 channels (got {c})")
+    if not eps >= 0:
+        raise ValueError(f"layer_norm: eps must not be negative (got {eps})")
+    _need_gpu("layer_norm", x, weight, bias)
+    return _apply(_LayerNorm, x, weight, bias, float(eps), -1 if axis == nd - 1 else 1)
+
+
+# ------------------------------------------------------------------------------ token log probabilities
+class LogProbs(NamedTuple):
+    """What :func:`log_probs` returns; ``top_log_probs`` and ``top_indices`` have top_k entries in the class axis's place."""
+    log_prob: torch.Tensor
+    entropy: torch.Tensor
+    top_log_probs: torch.Tensor
+    top_indices: torch.Tensor
+
+
+class _LogProbs(torch.autograd.Function):
+    """x: [outer, V] with contiguous classes (inner = 1) or dense [outer, V, inner]; target [outer * inner]."""
+
+    @staticmethod
+    def forward(ctx, x, target, top_k, ignore_index):
+        outer, v = x.shape[0], x.shape[1]
+        inner = x.shape[2] if x.dim() == 3 else 1
+        tail = (inner,) if x.dim() == 3 else ()
+        dev = x.device
+        n = outer * inner
+        # log_prob, entropy and the kept (maximum, log sum) in one allocation
+        flat = torch.empty(4 * n, dtype=torch.float32, device=dev)
+        lp, ent, stats = flat[:n], flat[n:2 * n], flat[2 * n:]
+        top = torch.empty((outer, top_k) + tail, dtype=torch.float32, device=dev)
+        idx = torch.empty((outer, top_k) + tail, dtype=torch.int64, device=dev)
+        ld = x.stride(0) if outer > 1 else v
+        lib = _lib.lib()
+        n_ws = lib.erf_log_probs_workspace_bytes(outer, v, inner, top_k)
+        ws = torch.empty(n_ws, dtype=torch.uint8, device=dev) if n_ws else None
+        with _dev_ctx(x):
+            _lib.check(_fn("erf_log_probs_forward", x)(
+                _p(x), _p(target), _p(lp), _p(ent), _p(stats), _p(top), _p(idx), outer, v, inner, ld, top_k, ignore_index,
+                _p(ws), n_ws, _stream(x)))
+        ctx.mark_non_differentiable(idx)
+        if ctx.needs_input_grad[0]:
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(x, target, stats, ent, idx)
+            ctx.cfg = (outer, v, inner, ld, top_k, ignore_index)
+        return lp, ent, top, idx
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_lp, g_ent, g_top, _):
+        x, target, stats, ent, idx = ctx.saved_tensors
+        outer, v, inner, ld, top_k, ignore_index = ctx.cfg
+        g_lp, g_ent, g_top = (None if g is None else g.to(torch.float32).contiguous() for g in (g_lp, g_ent, g_top))
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        with _dev_ctx(x):
+            _lib.check(_fn("erf_log_probs_backward", x)(
+                _p(x), _p(target), _p(ent), _p(stats), _p(idx), _p(g_lp), _p(g_ent), _p(g_top), _p(dx), outer, v, inner, ld,
+                top_k, ignore_index, _stream(x)))
+        return dx, None, None, None
+
+
+def log_probs(logits, target, top_k=0, dim=-1, ignore_index=-1):
+    """Log probability of the given classes, entropy, and the ``top_k`` likeliest alternatives with their log
+    probabilities, of softmax(logits) over ``dim``, differentiable in all three; see :class:`LogProbs`.
+
+    logits fp32 or bf16 (results are fp32); target int64 of logits' shape without ``dim``.  A target that is
+    ``ignore_index`` or no class gives log_prob 0 and passes no gradient.  0 <= top_k <= min(64, classes); alternatives
+    come largest first, equal logits by index.  Classes masked with -infinity have probability 0; a row of nothing else
+    has log probabilities of -infinity, entropy 0 and no gradient.  A NaN or +infinity makes its row NaN.
+
+    Rows of contiguous classes (the last axis, also with a stride between rows) and pixels ([N,K,H,W], dim 1) are read in
+    place; other layouts are copied into rows first.  The reference has only the mean of the first result
+    (CrossEntropyLoss2d, train/evaluation_functions.py:6-14)."""
+    _check_act(logits)
+    nd = logits.dim()
+    if nd < 1 or not -nd <= dim < nd:
+        raise ValueError(f"log_probs: dim {dim} of logits {tuple(logits.shape)}")
+    axis = dim + nd if dim < 0 else dim
+    shape = tuple(logits.shape)
+    lead, v, tail = shape[:axis], shape[axis], shape[axis + 1:]
+    if target.dtype != torch.int64:
+        raise TypeError(f"log_probs: target must be int64 class indices, got {target.dtype}")
+    if tuple(target.shape) != lead + tail:
+        raise ValueError(f"log_probs: target shape {tuple(target.shape)} does not match logits {shape} without dim {dim}")
+    if not 1 <= v <= 1 << 30:
+        raise ValueError(f"log_probs: 1..{1 << 30} classes (got {v})")
+    if not 0 <= top_k <= min(64, v):
+        raise ValueError(f"log_probs: top_k must be in 0..{min(64, v)} (got {top_k})")
+    _need_gpu("log_probs", logits, target)
+    _materialize_logits(logits)
+    inner = 1
+    for s in tail:
+        inner *= s
+    outer = logits.numel() // (v * inner) if inner else 0
+    tg = target.contiguous().view(-1)
+    # The pixel kernel gives a thread a pixel; it needs enough of them to fill the card, and keeps up to 8
+    # alternatives in registers.
+    if inner > 1 and v <= 256 and top_k <= 8 and outer * inner >= 4096:
+        x = logits.contiguous().view(outer, v, inner)
+        lp, ent, top, idx = _apply(_LogProbs, x, tg, int(top_k), int(ignore_index))
+        full = lead + (top_k,) + tail
+        return LogProbs(lp.view(target.shape), ent.view(target.shape), top.view(full), idx.view(full))
+    x = (logits if axis == nd - 1 else logits.movedim(axis, -1)).reshape(-1 if v * inner else 0, v)
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < v):
+        x = x.contiguous()
+    lp, ent, top, idx = _apply(_LogProbs, x, tg, int(top_k), int(ignore_index))
+    full = lead + tail + (top_k,)
+    top, idx = top.view(full), idx.view(full)
+    if axis != nd - 1:
+        top, idx = top.movedim(-1, axis), idx.movedim(-1, axis)
+    return LogProbs(lp.view(target.shape), ent.view(target.shape), top, idx)

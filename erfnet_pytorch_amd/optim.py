@@ -18,7 +18,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["Adam", "SGD"]
+__all__ = ["Adam", "SGD", "AdamW"]
 
 
 class _Tables:
@@ -40,12 +40,13 @@ class _Tables:
         return self.ptrs, self.numel
 
 
-def _usable(p, what):
+def _usable(p, what, dtypes=(torch.float32,)):
     if not p.is_cuda:
         raise RuntimeError(f"erfnet_pytorch_amd.optim: {what} lives on {p.device}; the update kernels "
                            "run on the GPU only (use torch.optim for host tensors)")
-    if p.dtype != torch.float32:
-        raise TypeError(f"erfnet_pytorch_amd.optim: {what} is {p.dtype}; parameters and gradients are fp32")
+    if p.dtype not in dtypes:
+        raise TypeError(f"erfnet_pytorch_amd.optim: {what} is {p.dtype}; parameters and gradients are " +
+                        ("fp32" if dtypes == (torch.float32,) else "fp32 or bf16, one type for both"))
     if not p.is_contiguous():
         raise ValueError(f"erfnet_pytorch_amd.optim: {what} is not contiguous")
 
@@ -154,4 +155,98 @@ class SGD(torch.optim.Optimizer):
                 _lib.check(lib.erf_sgd_step(
                     len(ps), ptrs[0], ptrs[1], ptrs[2], numel, float(group["lr"]), float(group["momentum"]),
                     float(group["weight_decay"]), C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)))
+        return loss
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` (no amsgrad, no maximize) for fp32 and bf16 parameters, one launch per 56 tensors.
+
+    ``state_bits=32``: fp32 moments under torch's key names, so that state dicts travel between the two classes.
+    ``state_bits=8``: both moments as float8 (e4m3) with one fp32 scale per 256 consecutive elements — ``exp_avg``,
+    ``exp_avg_scale`` and, as the square root of the second moment, ``exp_avg_sq_root``, ``exp_avg_sq_root_scale`` (value =
+    code * scale): 2 bytes an element held instead of 8.  The update itself uses the moments before they are
+    rounded.  ``load_state_dict`` takes the state of an optimiser with the same ``state_bits`` only.
+
+    ``step`` cannot be captured into a HIP graph: the bias corrections of the step go into the launch."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
+        if lr < 0.0 or eps < 0.0 or weight_decay < 0.0:
+            raise ValueError("AdamW: lr, eps and weight_decay must not be negative")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"AdamW: betas {betas} outside [0, 1)")
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 8 or 32 (got {state_bits})")
+        self.state_bits = state_bits
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False,
+                                      maximize=False, foreach=None, capturable=False, differentiable=False,
+                                      fused=None, decoupled_weight_decay=True))
+        self._tables = {}
+
+    @property
+    def _moments(self):
+        """State keys in the order of the library's pointer tables."""
+        return ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else \
+            ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale")
+
+    def _new_state(self, p):
+        if self.state_bits == 32:
+            return {k: torch.zeros_like(p, dtype=torch.float32) for k in self._moments}
+        scales = -(-p.numel() // 256)
+        return {k: torch.zeros(scales, dtype=torch.float32, device=p.device) if k.endswith("_scale") else
+                torch.zeros_like(p, dtype=torch.float8_e4m3fn) for k in self._moments}
+
+    def load_state_dict(self, state_dict):
+        want = set(self._moments)
+        for st in state_dict["state"].values():
+            if set(st) - {"step"} != want:
+                raise ValueError(f"AdamW(state_bits={self.state_bits}): the state dict holds {sorted(st)}, not "
+                                 f"step and {sorted(want)}")
+        super().load_state_dict(state_dict)
+        # torch casts floating-point state to the parameter's type; the moments keep their own
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+            for k in want if i in state_dict["state"] else ():
+                self.state[p][k] = state_dict["state"][i][k].detach().to(p.device, copy=True)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        lib = _lib.lib()
+        for gi, group in enumerate(self.param_groups):
+            if group.get("amsgrad") or group.get("maximize") or not group.get("decoupled_weight_decay", True):
+                raise NotImplementedError("erfnet_pytorch_amd.optim.AdamW: amsgrad / maximize / L2 weight decay are "
+                                          "not implemented (Adam has the latter)")
+            lists = {}
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if g.is_sparse:
+                    raise RuntimeError("erfnet_pytorch_amd.optim: sparse gradients are not supported")
+                _usable(p, "a parameter", (torch.float32, torch.bfloat16))
+                _usable(g, "a gradient", (p.dtype,))
+                st = self.state[p]
+                if not st:
+                    st["step"] = torch.tensor(0.0)
+                    st.update(self._new_state(p))
+                lists.setdefault((p.device, p.dtype, int(st["step"])), []).append((p, g, st))
+            for li, ((dev, dtype, step), items) in enumerate(lists.items()):
+                with torch.cuda.device(dev):
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("erfnet_pytorch_amd.optim.AdamW: step() cannot be captured into a graph")
+                    tensors = [[p for p, _, _ in items], [g for _, g, _ in items]]
+                    tensors += [[st[k] for _, _, st in items] for k in self._moments]
+                    tab = self._tables.setdefault((gi, li), _Tables(len(tensors)))
+                    ptrs, numel = tab.update(tensors)
+                    fn = getattr(lib, ("erf_adamw_step" if self.state_bits == 32 else "erf_adamw8_step") +
+                                 ("_bf16" if dtype == torch.bfloat16 else ""))
+                    b1, b2 = group["betas"]
+                    _lib.check(fn(len(items), *ptrs, numel, float(group["lr"]), float(b1), float(b2),
+                                  float(group["eps"]), float(group["weight_decay"]), step + 1,
+                                  C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)))
+                for _, _, st in items:
+                    st["step"] = torch.tensor(float(step + 1))
         return loss

@@ -51,7 +51,7 @@ typedef struct {
  * changed erf_nb1d_block_t's member types, 102 added ERF_OPT_X3_ROLL and the capture rule of
  * erf_cross_entropy_forward_static, 103 added erf_nb1d_block_t::sign_bits / sign_bits_written and
  * erf_nb1d_backward_bits, 104 the erf_batch_* calls, 105 ERF_OPT_POOL_FUSE). */
-#define ERF_ABI_VERSION 105
+#define ERF_ABI_VERSION 106
 int erf_version(void);
 const char *erf_last_error(void);
 /* Number of kernel launches issued through this library by the calling process (tests use it to
@@ -321,6 +321,43 @@ int erf_cross_entropy_backward(const float *logits, const long long *target, con
                                const float *stats, const float *gy, float *dlogits, int N, int K, int H,
                                int W, long long ignore_index, void *stream);
 
+/* ---- Layer norm over the last axis of dense rows [rows][C], 1 <= C <= 16384 (no counterpart in the reference, whose
+ * blocks normalise over the batch; the channel vector of an NHWC pixel is such a row).  y = (x - mean) / sqrt(var + eps)
+ * * w + b with the biased variance of the row; w, b: [C] fp32 or NULL (1 and 0).  mean, rstd: fp32 [rows], kept for
+ * backward, or both NULL.  Backward: dx (may be NULL), dw and db (each may be NULL; zeros when rows = 0); ws:
+ * erf_layer_norm_workspace_bytes(rows, C), needed for dw / db only.  Every sum runs in a fixed order. */
+size_t erf_layer_norm_workspace_bytes(long long rows, int C);
+int erf_layer_norm_forward(const float *x, const float *w, const float *b, float *y, float *mean, float *rstd,
+                           long long rows, int C, float eps, void *stream);
+int erf_layer_norm_backward(const float *x, const float *w, const float *mean, const float *rstd, const float *gy,
+                            float *dx, float *dw, float *db, long long rows, int C, void *ws, size_t ws_bytes,
+                            void *stream);
+
+/* ---- Log probabilities of given classes, entropy and likeliest alternatives of a softmax (beside
+ * erf_cross_entropy_forward, which returns only their mean over pixels) --------------------------------------------------
+ * logits: [outer][V][inner].  inner = 1: rows of V contiguous classes, row_stride elements apart (>= V); inner > 1: dense,
+ * the NCHW pixel layout (row_stride is ignored).  target: int64 [outer][inner]; a label that is ignore_index or outside
+ * [0, V) gets log_prob 0 and passes no gradient.
+ *   log_prob [outer][inner] = log p[target];  entropy [outer][inner] = -sum p log p;
+ *   top_log_probs / top_indices [outer][top_k][inner]: the top_k largest, equal ones by index; top_k <= V and
+ *   <= ERF_LOG_PROBS_MAX_TOP (inner = 1) or ERF_LOG_PROBS_MAX_TOP_PIXELS; both may be NULL for top_k = 0;
+ *   stats [outer][inner][2]: maximum and log of the sum of exponentials above it, for backward.
+ * Logits of -infinity have probability 0; a row of nothing else has log probabilities of -infinity, entropy 0 and no
+ * gradient.  NaN or +infinity makes its row NaN.  ws: erf_log_probs_workspace_bytes().
+ * Backward: g_log_prob, g_entropy [outer][inner] and g_top [outer][top_k][inner], each may be NULL (zero); dlogits is dense
+ * [outer][V][inner]. */
+#define ERF_LOG_PROBS_MAX_TOP 64
+#define ERF_LOG_PROBS_MAX_TOP_PIXELS 8
+size_t erf_log_probs_workspace_bytes(long long outer, int V, long long inner, int top_k);
+int erf_log_probs_forward(const float *logits, const long long *target, float *log_prob, float *entropy, float *stats,
+                          float *top_log_probs, long long *top_indices, long long outer, int V, long long inner,
+                          long long row_stride, int top_k, long long ignore_index, void *ws, size_t ws_bytes,
+                          void *stream);
+int erf_log_probs_backward(const float *logits, const long long *target, const float *entropy, const float *stats,
+                           const long long *top_indices, const float *g_log_prob, const float *g_entropy,
+                           const float *g_top, float *dlogits, long long outer, int V, long long inner,
+                           long long row_stride, int top_k, long long ignore_index, void *stream);
+
 /* ---- masked regression losses (train/evaluation_functions.py:32-97; train/main.py:173-184) ------
  * The mean, over the pixels whose float target is not -1, of a per-pixel value:
  *   kind 0  L1LossMasked (:89-97)                      |a - t|                         K = 1
@@ -389,6 +426,20 @@ int erf_sgd_step(int count, float *const *params, const float *const *grads, flo
                  const long long *numel, double lr, double momentum, double weight_decay, void *stream);
 int erf_ema_update(int count, float *const *target, const float *const *source, const long long *numel,
                    double discount, void *stream);
+
+/* AdamW (weight decay taken off the parameter, not added to the gradient) over many tensors; arguments as erf_adam_step.
+ * erf_adamw8_step keeps the moments in 8 bits: exp_avg and the square ROOT of exp_avg_sq as float8 e4m3 codes (numel bytes
+ * each) with one fp32 scale per 256 consecutive elements of a tensor (ceil(numel / 256) scales; value = code * scale,
+ * scale = the block's largest magnitude / 448; all zeros is the state before the first step).  The update itself uses the
+ * moments before they are rounded.  A nonzero root is never stored as zero; NaN and infinity are stored as NaN in their
+ * own element; a block whose largest magnitude is below 2^-100 is stored as zeros. */
+int erf_adamw_step(int count, float *const *params, const float *const *grads, float *const *exp_avg,
+                   float *const *exp_avg_sq, const long long *numel, double lr, double beta1, double beta2,
+                   double eps, double weight_decay, long long step, void *stream);
+int erf_adamw8_step(int count, float *const *params, const float *const *grads, void *const *exp_avg,
+                    float *const *exp_avg_scale, void *const *exp_avg_sq_root, float *const *exp_avg_sq_root_scale,
+                    const long long *numel, double lr, double beta1, double beta2, double eps, double weight_decay,
+                    long long step, void *stream);
 
 /* ================================================================================================
  * bf16 storage.  Every block call above exists a second time, suffixed _bf16, for activation tensors
@@ -477,6 +528,30 @@ int erf_conv2d_forward_bf16(const void *x, const float *w, const float *b, void 
 int erf_conv2d_backward_bf16(const void *x, const float *w, const void *y, const void *gy, void *dx,
                              float *dw, float *db, int N, int Cin, int H, int W, int Cout, int k,
                              int relu, void *ws, size_t ws_bytes, void *stream);
+
+/* Layer norm: x, y, gy, dx bf16.  Log probabilities: logits, dlogits bf16 (every other tensor stays fp32 / int64).  AdamW:
+ * params and grads bf16, moments as above. */
+int erf_layer_norm_forward_bf16(const void *x, const float *w, const float *b, void *y, float *mean, float *rstd,
+                                long long rows, int C, float eps, void *stream);
+int erf_layer_norm_backward_bf16(const void *x, const float *w, const float *mean, const float *rstd,
+                                 const void *gy, void *dx, float *dw, float *db, long long rows, int C, void *ws,
+                                 size_t ws_bytes, void *stream);
+int erf_log_probs_forward_bf16(const void *logits, const long long *target, float *log_prob, float *entropy,
+                               float *stats, float *top_log_probs, long long *top_indices, long long outer, int V,
+                               long long inner, long long row_stride, int top_k, long long ignore_index, void *ws,
+                               size_t ws_bytes, void *stream);
+int erf_log_probs_backward_bf16(const void *logits, const long long *target, const float *entropy,
+                                const float *stats, const long long *top_indices, const float *g_log_prob,
+                                const float *g_entropy, const float *g_top, void *dlogits, long long outer, int V,
+                                long long inner, long long row_stride, int top_k, long long ignore_index,
+                                void *stream);
+int erf_adamw_step_bf16(int count, void *const *params, const void *const *grads, float *const *exp_avg,
+                        float *const *exp_avg_sq, const long long *numel, double lr, double beta1, double beta2,
+                        double eps, double weight_decay, long long step, void *stream);
+int erf_adamw8_step_bf16(int count, void *const *params, const void *const *grads, void *const *exp_avg,
+                         float *const *exp_avg_scale, void *const *exp_avg_sq_root, float *const *exp_avg_sq_root_scale,
+                         const long long *numel, double lr, double beta1, double beta2, double eps,
+                         double weight_decay, long long step, void *stream);
 
 #ifdef __cplusplus
 }
