@@ -28,7 +28,7 @@ int log2_up(int v)
 
 // ================================================================================ layer norm
 // A row of up to 16 elements a lane and 64 lanes stays inside a wave (no barrier, several short rows a wave);
-// longer rows take a block, one to four vectors a thread.
+// longer rows take a block of up to 1024 threads with 16 elements each.
 struct NormPlan {
     bool wave;
     int rounds, lanes, threads;
@@ -43,16 +43,20 @@ template <typename T> NormPlan norm_plan(int C)
         return p;
     }
     p.wave = false;
-    while (p.rounds * 1024 < vecs) p.rounds *= 2;
-    p.threads = ((vecs + p.rounds - 1) / p.rounds + 63) / 64 * 64;
+    p.rounds = most;
+    p.threads = ((vecs + most - 1) / most + 63) / 64 * 64;
     return p;
 }
-int norm_blocks(const NormPlan &p, long long rows, int most)
+// Blocks that walk over the rows: as many as the card holds at once, `threads` of them on a compute unit.  Backward takes
+// at least `turns` rows a thread beyond one block per unit, so that the blocks' partial sums stay a small part of its traffic.
+int norm_blocks(const NormPlan &p, long long rows, int threads, int turns)
 {
     const long long per = p.wave ? NORM_BLOCK / p.lanes : 1;
-    return (int)std::min<long long>((rows + per - 1) / per, most);
+    const long long all = (rows + per - 1) / per, full = 256ll * std::max(1, threads / p.threads);
+    return (int)std::min(std::min(all, full), std::max<long long>(256, all / turns));
 }
-#define NORM_BWD_BLOCKS(p) ((p).wave ? 1024 : (p).threads > 512 ? 256 : 512)
+#define NORM_FWD_BLOCKS(p, rows) norm_blocks(p, rows, 2048, 1)
+#define NORM_BWD_BLOCKS(p, rows) norm_blocks(p, rows, 1024, 8)
 
 int norm_check(const char *what, const void *x, const void *y, long long rows, int C, float eps)
 {
@@ -75,25 +79,20 @@ int norm_forward(const void *x, const float *w, const float *b, void *y, float *
     memset(&d, 0, sizeof(d));
     d.x = x; d.y = y; d.w = w; d.b = b; d.mean = mean; d.rstd = rstd;
     d.rows = rows; d.C = C; d.eps = eps; d.lanes = p.lanes; d.lane_bits = log2_up(p.lanes);
-    const int blocks = norm_blocks(p, rows, 2048);
-    if (p.wave) {
-        if (p.rounds == 1) norm_fwd_wave_kernel<T, 1><<<blocks, NORM_BLOCK, 0, st>>>(d);
-        else if (p.rounds == 2) norm_fwd_wave_kernel<T, 2><<<blocks, NORM_BLOCK, 0, st>>>(d);
-        else if constexpr (Vec16<T>::N == 4) norm_fwd_wave_kernel<T, 4><<<blocks, NORM_BLOCK, 0, st>>>(d);
-        LAUNCHED("norm_fwd_wave_kernel");
-        return 0;
-    }
-    if (p.rounds == 1) norm_fwd_block_kernel<T, 1><<<blocks, p.threads, 0, st>>>(d);
-    else if (p.rounds == 2) norm_fwd_block_kernel<T, 2><<<blocks, p.threads, 0, st>>>(d);
-    else if constexpr (Vec16<T>::N == 4) norm_fwd_block_kernel<T, 4><<<blocks, p.threads, 0, st>>>(d);
-    LAUNCHED("norm_fwd_block_kernel");
+    const int blocks = NORM_FWD_BLOCKS(p, rows);
+    constexpr int most = 16 / Vec16<T>::N;
+    if (!p.wave) norm_fwd_kernel<T, most, true><<<blocks, p.threads, 0, st>>>(d);
+    else if (p.rounds == 1) norm_fwd_kernel<T, 1, false><<<blocks, NORM_BLOCK, 0, st>>>(d);
+    else if (p.rounds == 2) norm_fwd_kernel<T, 2, false><<<blocks, NORM_BLOCK, 0, st>>>(d);
+    else norm_fwd_kernel<T, most, false><<<blocks, NORM_BLOCK, 0, st>>>(d);
+    LAUNCHED("norm_fwd_kernel");
     return 0;
 }
 
 template <typename T> size_t norm_ws(long long rows, int C)
 {
     const NormPlan p = norm_plan<T>(C);
-    return (size_t)norm_blocks(p, rows, NORM_BWD_BLOCKS(p)) * 2 * C * sizeof(float);
+    return (size_t)NORM_BWD_BLOCKS(p, rows) * 2 * C * sizeof(float);
 }
 
 template <typename T>
@@ -105,7 +104,8 @@ int norm_backward(const void *x, const float *w, const float *mean, const float 
     if (rows && (!mean || !rstd)) return fail("layer norm backward: null pointer");
     if (!dx && !params) return 0;
     const NormPlan p = norm_plan<T>(C);
-    const int blocks = norm_blocks(p, rows, NORM_BWD_BLOCKS(p));
+    const int blocks = NORM_BWD_BLOCKS(p, rows);
+    constexpr int most = 16 / Vec16<T>::N;
     NormDesc d;
     memset(&d, 0, sizeof(d));
     d.x = x; d.gy = gy; d.y = dx; d.w = w; d.mean = const_cast<float *>(mean); d.rstd = const_cast<float *>(rstd);
@@ -115,21 +115,16 @@ int norm_backward(const void *x, const float *w, const float *mean, const float 
         d.partial = (float *)ws;
     }
     if (blocks) {
-        if (p.wave) {
-            const size_t lds = params ? (size_t)8 * C * sizeof(float) : 0;
-            if (p.rounds == 1) norm_bwd_wave_kernel<T, 1><<<blocks, NORM_BLOCK, lds, st>>>(d);
-            else if (p.rounds == 2) norm_bwd_wave_kernel<T, 2><<<blocks, NORM_BLOCK, lds, st>>>(d);
-            else if constexpr (Vec16<T>::N == 4) norm_bwd_wave_kernel<T, 4><<<blocks, NORM_BLOCK, lds, st>>>(d);
-            LAUNCHED("norm_bwd_wave_kernel");
-        } else {
-            if (p.rounds == 1) norm_bwd_block_kernel<T, 1><<<blocks, p.threads, 0, st>>>(d);
-            else if (p.rounds == 2) norm_bwd_block_kernel<T, 2><<<blocks, p.threads, 0, st>>>(d);
-            else if constexpr (Vec16<T>::N == 4) norm_bwd_block_kernel<T, 4><<<blocks, p.threads, 0, st>>>(d);
-            LAUNCHED("norm_bwd_block_kernel");
-        }
+        const size_t lds = params && p.wave ? (size_t)8 * C * sizeof(float) : 0;
+        if (!p.wave && p.threads > 512) norm_bwd_kernel<T, most, 1024><<<blocks, p.threads, 0, st>>>(d);
+        else if (!p.wave) norm_bwd_kernel<T, most, 512><<<blocks, p.threads, 0, st>>>(d);
+        else if (p.rounds == 1) norm_bwd_kernel<T, 1, 0><<<blocks, NORM_BLOCK, lds, st>>>(d);
+        else if (p.rounds == 2) norm_bwd_kernel<T, 2, 0><<<blocks, NORM_BLOCK, lds, st>>>(d);
+        else norm_bwd_kernel<T, most, 0><<<blocks, NORM_BLOCK, lds, st>>>(d);
+        LAUNCHED("norm_bwd_kernel");
     }
     if (params) {
-        norm_grad_sum_kernel<<<(2 * C + 31) / 32, 1024, 0, st>>>((const float *)ws, blocks, C, dw, db);   // (no rows: zeros)
+        norm_grad_sum_kernel<<<(2 * C + 15) / 16, 1024, 0, st>>>((const float *)ws, blocks, C, dw, db);   // (no rows: zeros)
         LAUNCHED("norm_grad_sum_kernel");
     }
     return 0;

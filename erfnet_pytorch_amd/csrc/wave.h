@@ -1,0 +1,47 @@
+// Reductions over neighbouring lanes of a wave without shared memory (data-parallel primitives and the gfx950 lane swaps).
+#pragma once
+#include "common.h"
+
+template <int CTRL> __device__ __forceinline__ float wave_dpp(float v)
+{
+    const int i = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ void wave_halves(float v, float &a, float &b)        // lanes 0..31 and 32..63, to both halves
+{
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned x = r[0], y = r[1];
+    a = __builtin_bit_cast(float, x);
+    b = __builtin_bit_cast(float, y);
+}
+__device__ __forceinline__ void wave_rows(float v, float &a, float &b)          // rows of 16: each pair's first and second
+{
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned x = r[0], y = r[1];
+    a = __builtin_bit_cast(float, x);
+    b = __builtin_bit_cast(float, y);
+}
+
+// Sum (or maximum) over aligned groups of `lanes` lanes, a power of two up to 64; every lane gets its group's.  A step
+// joins the two halves of a group that are each uniform already, so a mirror does for an exchange.
+template <typename F> __device__ __forceinline__ float wave_reduce(float v, int lanes, F join)
+{
+    float a, b;
+    if (lanes > 1) v = join(v, wave_dpp<0xb1>(v));          // quad_perm 1,0,3,2
+    if (lanes > 2) v = join(v, wave_dpp<0x4e>(v));          // quad_perm 2,3,0,1
+    if (lanes > 4) v = join(v, wave_dpp<0x141>(v));         // mirror within 8
+    if (lanes > 8) v = join(v, wave_dpp<0x140>(v));         // mirror within 16
+    if (lanes > 16) { wave_rows(v, a, b); v = join(a, b); }
+    if (lanes > 32) { wave_halves(v, a, b); v = join(a, b); }
+    return v;
+}
+__device__ __forceinline__ float wave_sum(float v, int lanes = 64)
+{
+    return wave_reduce(v, lanes, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_max(float v, int lanes = 64)
+{
+    return wave_reduce(v, lanes, [](float a, float b) { return fmaxf(a, b); });
+}
