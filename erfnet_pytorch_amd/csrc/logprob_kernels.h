@@ -12,6 +12,7 @@
 // Alternatives are ordered by logit, larger first, NaN before all, equal ones by index: one 64-bit key per entry.
 #pragma once
 #include "vec16.h"
+#include "wave.h"
 
 #define LP_BLOCK 256
 #define LP_MAX_TOP 64
@@ -81,66 +82,68 @@ __device__ __forceinline__ void lp_join(LpSums &r, LpSums o)
     r.a += o.a;
 }
 
-// ---------------------------------------------------------------------------------- a wave's list of the largest keys
-// Lane i of `list` holds the i-th largest key seen so far (0: none).  New candidates gather in 64 slots of shared
-// memory; a full buffer is sorted and merged into the list (bitonic networks over the lanes).
-__device__ __forceinline__ unsigned long long lp_shfl_xor(unsigned long long v, int o)
+// ---------------------------------------------------------------------------------- the largest keys
+// The scan itself looks for no alternatives: it leaves every thread with its maximum, and the k-th largest of those is a
+// bar that at least k entries reach.  Only threads whose maximum reaches it can hold an alternative, about k of them, and only
+// their entries are read again.  (Filtering entries against a running bar inside the scan took 240 us for 2047 rows of
+// 100003 bf16 classes, k = 8; the scan alone takes 100.)
+//
+// Sorting networks over the 64 lanes, larger values in lower lanes.
+template <int O> __device__ __forceinline__ unsigned lp_xor(unsigned v) { return wave_xor<O>(v); }
+template <int O> __device__ __forceinline__ unsigned long long lp_xor(unsigned long long v)
 {
-    const unsigned lo = __shfl_xor((unsigned)v, o), hi = __shfl_xor((unsigned)(v >> 32), o);
-    return (unsigned long long)hi << 32 | lo;
+    return (unsigned long long)wave_xor<O>((unsigned)(v >> 32)) << 32 | wave_xor<O>((unsigned)v);
 }
-__device__ __forceinline__ unsigned long long lp_shfl(unsigned long long v, int src)
+__device__ __forceinline__ unsigned lp_reverse(unsigned v) { return wave_reverse(v); }
+__device__ __forceinline__ unsigned long long lp_reverse(unsigned long long v)
 {
-    const unsigned lo = __shfl((unsigned)v, src), hi = __shfl((unsigned)(v >> 32), src);
-    return (unsigned long long)hi << 32 | lo;
+    return (unsigned long long)wave_reverse((unsigned)(v >> 32)) << 32 | wave_reverse((unsigned)v);
 }
-// descending over the lanes from a bitonic sequence
-__device__ __forceinline__ unsigned long long lp_bitonic_clean(unsigned long long v)
+// descending over aligned groups of 2 * O lanes, from bitonic sequences; `turn`: ascending instead
+template <int O, typename K> __device__ __forceinline__ K lp_clean(K v, bool turn)
 {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned long long w = lp_shfl_xor(v, o);
-        const bool keep_max = (lane & o) == 0;
-        v = (v > w) == keep_max ? v : w;
-    }
+    const K w = lp_xor<O>(v);
+    const bool keep_max = ((threadIdx.x & O) == 0) != turn;
+    v = (v > w) == keep_max ? v : w;
+    if constexpr (O > 1) return lp_clean<O / 2>(v, turn);
     return v;
 }
-__device__ __forceinline__ unsigned long long lp_sort64(unsigned long long v)
+template <typename K> __device__ __forceinline__ K lp_sort64(K v)
 {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-        for (int o = size >> 1; o > 0; o >>= 1) {
-            const unsigned long long w = lp_shfl_xor(v, o);
-            const bool keep_max = ((lane & o) == 0) == ((lane & size) == 0);
-            v = (v > w) == keep_max ? v : w;
-        }
-    return v;
+    const unsigned lane = threadIdx.x & 63;
+    v = lp_clean<1>(v, lane & 2);
+    v = lp_clean<2>(v, lane & 4);
+    v = lp_clean<4>(v, lane & 8);
+    v = lp_clean<8>(v, lane & 16);
+    v = lp_clean<16>(v, lane & 32);
+    return lp_clean<32>(v, false);
 }
 // both descending; the 64 largest of the 128
-__device__ __forceinline__ unsigned long long lp_merge(unsigned long long list, unsigned long long other)
+template <typename K> __device__ __forceinline__ K lp_merge(K list, K other)
 {
-    const unsigned long long r = lp_shfl(other, 63 - (int)(threadIdx.x & 63));
-    return lp_bitonic_clean(list > r ? list : r);
+    const K r = lp_reverse(other);
+    return lp_clean<32>(list > r ? list : r, false);
 }
 
+// A wave's candidates: up to 64 wait in shared memory; a full buffer is sorted into `list` (lane i: the i-th largest so
+// far, 0: none), after which nothing below its k-th enters.
+// (pointers into shared memory say so: a plain volatile pointer is read by flat loads)
+typedef __attribute__((address_space(3))) volatile unsigned long long lp_lds64;
+typedef __attribute__((address_space(3))) volatile unsigned char lp_lds8;
 struct LpList {
     unsigned long long list = 0, kth = 0;
-    float bar = -INFINITY;      // a value below the k-th largest cannot enter (compared with !(x < bar): NaN passes)
-    int count = 0;              // candidates in the buffer
-    volatile unsigned long long *buf;
+    int count = 0;
+    bool sorted = false;        // whether list holds anything
+    lp_lds64 *buf;
 
     __device__ __forceinline__ void flush(int k)
     {
         const int lane = threadIdx.x & 63;
-        unsigned long long v = lane < count ? buf[lane] : 0ull;
-        list = lp_merge(list, lp_sort64(v));
-        kth = lp_shfl(list, k - 1);
-        // (uniform over the wave; an unfilled list lets everything through)
-        bar = kth ? lp_key_value((unsigned)(kth >> 32)) : -INFINITY;
-        if (bar != bar) bar = INFINITY;         // k NaNs so far: only another NaN passes the bar, and the key decides
+        const unsigned long long v = lp_sort64(lane < count ? buf[lane] : 0ull);
+        list = sorted ? lp_merge(list, v) : v;
+        sorted = true;
+        kth = (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(list >> 32), k - 1) << 32 |
+              (unsigned)__builtin_amdgcn_readlane((int)list, k - 1);
         count = 0;
     }
     // every lane offers one key (0: none)
@@ -161,48 +164,106 @@ struct LpList {
 };
 
 // ---------------------------------------------------------------------------------- rows: the class axis is the last
-// What one thread does with its share of elements [from, to) of a row: vectors `threads` apart.
-template <typename T, bool TOP>
-__device__ __forceinline__ LpSums lp_scan(const T *x, int from, int to, int me, int threads, int k, LpList &top)
+template <int N, int U> __device__ __forceinline__ void lp_add_vectors(LpSums &r, const float (&v)[U][N])
 {
-    constexpr int N = Vec16<T>::N;
+    float high = v[0][0];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < N; ++i) high = fmaxf(high, v[u][i]);
+    if (high > r.m) lp_move(r, high);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < N; ++i) lp_add(r, v[u][i]);
+}
+
+// What one thread does with its share of elements [from, to) of a row: 16 at a time in vectors `threads` apart, with the
+// next ones' loads in flight; the last turn, which may lack some, by itself.
+template <typename T>
+__device__ __forceinline__ LpSums lp_scan(const T *x, int from, int to, int me, int threads)
+{
+    constexpr int N = Vec16<T>::N, U = 16 / N;
     LpSums r = {LP_LOWEST, 0.0f, 0.0f};
-    // all lanes of a wave take every turn (the list's votes need them)
-    for (int base = from; base < to; base += threads * N) {
-        const int c = base + me * N;
-        const int left = to - c;
-        float v[N];
-        Vec16<T>::unpack(ld16(x + c, left), v);
-        if (left < N) {
+    const int step = threads * N, turns = (to - from) / (step * U);
+    const T *at = x + from + me * N;
+    u32x4 next[U];
+    float v[U][N];
+    auto fetch = [&]() __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = i < left ? v[i] : -INFINITY;
+        for (int u = 0; u < U; ++u) next[u] = reinterpret_cast<const typename Vec16<T>::Raw *>(at + u * step)->v;
+        at += step * U;
+    };
+    if (turns) fetch();
+    for (int t = 0; t < turns; ++t) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) Vec16<T>::unpack(next[u], v[u]);
+        if (t + 1 < turns) fetch();
+        lp_add_vectors(r, v);
+    }
+    const int c0 = from + turns * step * U + me * N;
+    if (c0 < to) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) next[u] = ld16(x + c0 + u * step, to - c0 - u * step);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            Vec16<T>::unpack(next[u], v[u]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[u][i] = c0 + u * step + i < to ? v[u][i] : -INFINITY;
         }
-        float m = r.m;
-#pragma unroll
-        for (int i = 0; i < N; ++i) m = fmaxf(m, v[i]);
-        if (m > r.m) lp_move(r, m);
-#pragma unroll
-        for (int i = 0; i < N; ++i) lp_add(r, v[i]);
-        if (TOP) {
-            float high = v[0];
-#pragma unroll
-            for (int i = 1; i < N; ++i) high = fmaxf(high, v[i]);
-            // (a NaN is lost by fmaxf but not by the sums)
-            if (__ballot(left > 0 && (!(high < top.bar) || r.s != r.s))) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) top.offer(i < left ? lp_key(v[i], c + i) : 0ull, k);
-            }
-        }
+        lp_add_vectors(r, v);
     }
     return r;
 }
 
+// The entries of this wave's threads that reach `bar`, into top.  `owner`: this thread may hold one.  A lane takes one
+// vector of one owner at a time, so that a few owners' long shares occupy the whole wave.
+template <typename T>
+__device__ __forceinline__ void lp_collect(const T *x, int from, int to, int first, int threads, bool owner, unsigned bar,
+                                           int k, lp_lds8 *owners, LpList &top)
+{
+    constexpr int N = Vec16<T>::N;
+    const int lane = threadIdx.x & 63, step = threads * N;
+    const unsigned long long mask = __ballot(owner);
+    if (owner) {
+        const int at = __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
+        owners[at] = (unsigned char)lane;
+    }
+    const int turns = (to - from + step - 1) / step, n = __popcll(mask) * turns;
+    for (int q0 = 0; q0 < n; q0 += 64) {        // (the same number of turns for all lanes: the votes need them)
+        const int q = q0 + lane, o = q < n ? q / turns : 0;
+        const int c = from + (q - o * turns) * step + (first + owners[o]) * N;
+        const int left = q < n ? to - c : 0;
+        float v[N];
+        Vec16<T>::unpack(ld16(x + c, left), v);
+        unsigned mine = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) mine |= (i < left) & (lp_key32(v[i]) >= bar) ? 1u << i : 0u;
+        while (__ballot(mine != 0u)) {          // one entry from each lane a turn, the lowest first
+            const int j = __ffs(mine) - 1;      // (-1: nothing left, the selection below gives any of them)
+            // element j by bit selection (written as ternaries it becomes an indexed register file)
+            unsigned f[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = __builtin_bit_cast(unsigned, v[i]);
+#pragma unroll
+            for (int half = N / 2; half > 0; half >>= 1) {
+                unsigned pick = (j & half) ? ~0u : 0u;
+                asm volatile("" : "+v"(pick));
+#pragma unroll
+                for (int i = 0; i < half; ++i) f[i] = (f[i] & ~pick) | (f[i + half] & pick);
+            }
+            top.offer(mine ? lp_key(__builtin_bit_cast(float, f[0]), c + j) : 0ull, k);
+            mine &= mine - 1u;
+        }
+    }
+}
+
 __device__ __forceinline__ LpSums lp_wave_join(LpSums r)
 {
-    for (int o = 32; o > 0; o >>= 1) {
-        LpSums q = {__shfl_xor(r.m, o), __shfl_xor(r.s, o), __shfl_xor(r.a, o)};
-        lp_join(r, q);
-    }
+    const float m = wave_max(r.m);
+    lp_move(r, m);
+    r.s = wave_sum(r.s);
+    r.a = wave_sum(r.a);
     return r;
 }
 
@@ -230,10 +291,14 @@ __device__ __forceinline__ void lp_write_row(const LpDesc &d, long long row, con
 }
 
 // GROUP = 64: a wave takes a row, four rows a block.  GROUP = 256: a block takes one of `splits` segments of a row.
+// (8 waves a SIMD: without the bound the scalar registers leave 7)
 template <typename T, int GROUP, bool TOP>
-__global__ __launch_bounds__(LP_BLOCK) void lp_rows_kernel(const LpDesc d)
+__global__ __launch_bounds__(LP_BLOCK, 8) void lp_rows_kernel(const LpDesc d)
 {
     __shared__ unsigned long long buf[TOP ? 4 : 1][64];
+    __shared__ unsigned high[TOP ? 4 : 1][64];
+    __shared__ unsigned char owners[TOP ? 4 : 1][64];
+    __shared__ int counts[4];
     __shared__ LpSums sums[4];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     long long row;
@@ -249,30 +314,60 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_rows_kernel(const LpDesc d)
         from = split * d.seg;
         to = from + d.seg < d.V ? from + d.seg : d.V;
     }
+    const T *x = (const T *)d.x + row * d.ld;
+    LpSums r = lp_scan<T>(x, from, to, me, GROUP);
     LpList top;
-    top.buf = buf[TOP ? wave : 0];
-    LpSums r = lp_scan<T, TOP>((const T *)d.x + row * d.ld, from, to, me, GROUP, d.k, top);
-    if (TOP) top.flush(d.k);
+    if (TOP) {
+        top.buf = (lp_lds64 *)buf[wave];
+        // a thread's largest key, or a bound below it: the sums are NaN where it holds a NaN (which the maximum does not
+        // show) or +infinity; 0 where it holds nothing
+        const bool spoilt = r.s != r.s;
+        const unsigned mine = from + me * Vec16<T>::N >= to ? 0u : spoilt ? lp_key32(INFINITY)
+                              : r.s == 0.0f ? lp_key32(-INFINITY) : lp_key32(r.m);
+        unsigned best = lp_sort64(mine);
+        if (GROUP == 256) {
+            high[wave][lane] = best;
+            __syncthreads();
+            for (int w = 1; w < 4; ++w) best = lp_merge(best, high[(wave + w) & 3][lane]);
+        }
+        const unsigned bar = (unsigned)__builtin_amdgcn_readlane((int)best, d.k - 1);
+        lp_collect<T>(x, from, to, GROUP == 256 ? wave * 64 : 0, GROUP, mine != 0u && (spoilt || mine >= bar), bar > 1u ? bar : 1u,
+                      d.k, (lp_lds8 *)owners[wave], top);
+    }
     r = lp_wave_join(r);
     if (GROUP == 64) {
+        if (TOP) top.flush(d.k);
         lp_write_row<T>(d, row, r, top.list);
         return;
     }
-    // the four waves: sums through shared memory, lists in two rounds of merging
-    if (lane == 0) sums[wave] = r;
-    if (TOP) {
-        volatile unsigned long long *l = buf[wave];
-        l[lane] = top.list;
-        __syncthreads();
-        if (wave < 2) {
-            top.list = lp_merge(top.list, ((volatile unsigned long long *)buf[wave + 2])[lane]);
-            l[lane] = top.list;
-        }
+    // the four waves' sums and candidates, through shared memory; the candidates are few enough for one sort as a rule
+    if (lane == 0) {
+        sums[wave] = r;
+        if (TOP) counts[wave] = top.sorted ? 64 + 1 : top.count;
     }
     __syncthreads();
+    if (TOP) {
+        const int n0 = counts[0], n1 = n0 + counts[1], n2 = n1 + counts[2], n3 = n2 + counts[3];
+        if (n3 <= 64) {
+            if (wave == 0) {
+                const int w = lane < n0 ? 0 : lane < n1 ? 1 : lane < n2 ? 2 : 3;
+                const int at = lane - (w == 0 ? 0 : w == 1 ? n0 : w == 2 ? n1 : n2);
+                top.list = lp_sort64(lane < n3 ? ((lp_lds64 *)buf[w])[at] : 0ull);
+            }
+        } else {
+            top.flush(d.k);
+            top.buf[lane] = top.list;
+            __syncthreads();
+            if (wave < 2) {
+                top.list = lp_merge(top.list, ((lp_lds64 *)buf[wave + 2])[lane]);
+                top.buf[lane] = top.list;
+            }
+            __syncthreads();
+            if (wave == 0) top.list = lp_merge(top.list, ((lp_lds64 *)buf[1])[lane]);
+        }
+    }
     if (wave != 0) return;
     for (int w = 1; w < 4; ++w) lp_join(r, sums[w]);
-    if (TOP) top.list = lp_merge(top.list, ((volatile unsigned long long *)buf[1])[lane]);
     if (d.splits == 1) {
         lp_write_row<T>(d, row, r, top.list);
         return;
@@ -282,31 +377,32 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_rows_kernel(const LpDesc d)
     if (lane < d.k) d.part_keys[at * d.k + lane] = top.list;
 }
 
-// Joins the segments of a row: one block a row.
-template <typename T>
-__global__ __launch_bounds__(LP_BLOCK) void lp_join_kernel(const LpDesc d)
+// Joins the segments of a row.  WAVES = 1: a wave takes a row and merges its few lists one after the other, four rows a
+// block; 16: a block takes a row, every wave merges each 16th list and four rounds join the waves'.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(WAVES == 1 ? LP_BLOCK : WAVES * 64) void lp_join_kernel(const LpDesc d)
 {
-    __shared__ unsigned long long buf[4][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const long long row = blockIdx.x;
+    __shared__ unsigned long long buf[WAVES][64];
+    const int wave = WAVES == 1 ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const long long row = WAVES == 1 ? (long long)blockIdx.x * (LP_BLOCK / 64) + (threadIdx.x >> 6) : blockIdx.x;
+    if (row >= d.rows) return;                  // (WAVES = 1 alone: no barrier below there)
     unsigned long long list = 0;
-    if (d.k) {
-        for (int s = wave; s < d.splits; s += 4) {
-            const unsigned long long o = lane < d.k ? d.part_keys[(row * d.splits + s) * d.k + lane] : 0ull;
-            list = lp_merge(list, o);
-        }
-        buf[wave][lane] = list;
-        __syncthreads();
-        if (wave == 0)
-            for (int w = 1; w < 4; ++w) list = lp_merge(list, buf[w][lane]);
-    }
-    if (wave != 0) return;
     LpSums r = {LP_LOWEST, 0.0f, 0.0f};
-    for (int s = lane; s < d.splits; s += 64) {
-        const float4 p = d.part[row * d.splits + s];
-        lp_join(r, LpSums{p.x, p.y, p.z});
+    if (wave == 0)
+        for (int s = lane; s < d.splits; s += 64) {
+            const float4 p = d.part[row * d.splits + s];
+            lp_join(r, LpSums{p.x, p.y, p.z});
+        }
+    if (d.k) {
+        for (int s = wave; s < d.splits; s += WAVES)
+            list = lp_merge(list, lane < d.k ? d.part_keys[(row * d.splits + s) * d.k + lane] : 0ull);
+        for (int half = WAVES / 2; half > 0; half >>= 1) {
+            if (wave >= half && wave < 2 * half) buf[wave][lane] = list;
+            __syncthreads();
+            if (wave < half) list = lp_merge(list, buf[wave + half][lane]);
+        }
     }
-    lp_write_row<T>(d, row, lp_wave_join(r), list);
+    if (wave == 0) lp_write_row<T>(d, row, lp_wave_join(r), list);
 }
 
 // ---------------------------------------------------------------------------------- backward over rows

@@ -133,26 +133,27 @@ int norm_backward(const void *x, const float *w, const float *mean, const float 
 // ================================================================================ token log probabilities
 #define LP_MAX_CLASSES (1 << 30)
 
-// Blocks per row: a wave takes a row of up to 2048 classes; longer ones take whole blocks, several when the rows alone
-// would leave compute units without work (about four blocks each), with at least 2048 classes in every block.
+// Blocks per row: a wave takes a row of up to 2048 classes; longer ones take whole blocks of at least 4096 classes, several to
+// a row until they fill the card twice (2048 are resident), or once where every block also finds alternatives
+// (2047 x 100003 bf16: 82 us with two rounds, 95 with one; with 8 alternatives 116 and 114, and 123 with four rounds).
 struct LpPlan {
     bool wave;
     int splits, seg;
 };
-LpPlan lp_plan(long long rows, int V)
+LpPlan lp_plan(long long rows, int V, int k)
 {
     LpPlan p = {V <= 2048, 1, V};
     if (p.wave) return p;
-    const long long want = (1024 + rows - 1) / std::max<long long>(rows, 1);
-    p.splits = (int)std::min<long long>(std::max<long long>(want, 1), (V + 2047) / 2048);
-    p.seg = ((V + p.splits - 1) / p.splits + 2047) / 2048 * 2048;
+    const long long want = ((k ? 2048 : 4096) + rows - 1) / std::max<long long>(rows, 1);
+    p.splits = (int)std::min<long long>(std::max<long long>(want, 1), (V + 4095) / 4096);
+    p.seg = ((V + p.splits - 1) / p.splits + 4095) / 4096 * 4096;
     p.splits = (V + p.seg - 1) / p.seg;
     return p;
 }
 size_t lp_ws(long long outer, int V, long long inner, int k)
 {
     if (inner > 1) return 0;
-    const LpPlan p = lp_plan(outer, V);
+    const LpPlan p = lp_plan(outer, V, k);
     return p.splits > 1 ? (size_t)outer * p.splits * (sizeof(float4) + (size_t)k * 8) : 0;
 }
 
@@ -194,7 +195,7 @@ int lp_forward(const void *x, const long long *target, float *log_prob, float *e
         LAUNCHED("lp_pixels_kernel");
         return 0;
     }
-    const LpPlan p = lp_plan(outer, V);
+    const LpPlan p = lp_plan(outer, V, k);
     d.splits = p.splits; d.seg = p.seg;
     if (p.splits > 1) {
         if (!ws || ws_bytes < lp_ws(outer, V, inner, k)) return fail("log_probs: workspace too small");
@@ -212,7 +213,8 @@ int lp_forward(const void *x, const long long *target, float *log_prob, float *e
     }
     LAUNCHED("lp_rows_kernel");
     if (p.splits > 1) {
-        lp_join_kernel<T><<<(unsigned)outer, LP_BLOCK, 0, st>>>(d);
+        if (p.splits <= 8) lp_join_kernel<T, 1><<<(unsigned)((outer + 3) / 4), LP_BLOCK, 0, st>>>(d);
+        else lp_join_kernel<T, 16><<<(unsigned)outer, 1024, 0, st>>>(d);
         LAUNCHED("lp_join_kernel");
     }
     return 0;

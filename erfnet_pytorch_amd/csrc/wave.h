@@ -24,6 +24,33 @@ __device__ __forceinline__ void wave_rows(float v, float &a, float &b)          
     b = __builtin_bit_cast(float, y);
 }
 
+// The value of lane (own ^ O).
+template <int O> __device__ __forceinline__ unsigned wave_xor(unsigned v)
+{
+    const int i = (int)v;
+    if (O == 1) return (unsigned)__builtin_amdgcn_update_dpp(i, i, 0xb1, 0xf, 0xf, false);
+    if (O == 2) return (unsigned)__builtin_amdgcn_update_dpp(i, i, 0x4e, 0xf, 0xf, false);
+    if (O == 4) {       // mirror within 8 (own ^ 7), then within 4 (own ^ 3)
+        const int m = __builtin_amdgcn_update_dpp(i, i, 0x141, 0xf, 0xf, false);
+        return (unsigned)__builtin_amdgcn_update_dpp(m, m, 0x1b, 0xf, 0xf, false);
+    }
+    if (O == 8) return (unsigned)__builtin_amdgcn_update_dpp(i, i, 0x128, 0xf, 0xf, false);     // rotate a row by 8
+    if (O == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        const unsigned first = r[0], second = r[1];
+        return (threadIdx.x & 16) ? first : second;
+    }
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const unsigned first = r[0], second = r[1];
+    return (threadIdx.x & 32) ? first : second;
+}
+// The value of lane (63 - own): mirrored within 16, then the rows and the halves exchanged.
+__device__ __forceinline__ unsigned wave_reverse(unsigned v)
+{
+    const int i = (int)v;
+    return wave_xor<32>(wave_xor<16>((unsigned)__builtin_amdgcn_update_dpp(i, i, 0x140, 0xf, 0xf, false)));
+}
+
 // Sum (or maximum) over aligned groups of `lanes` lanes, a power of two up to 64; every lane gets its group's.  A step
 // joins the two halves of a group that are each uniform already, so a mirror does for an exchange.
 template <typename F> __device__ __forceinline__ float wave_reduce(float v, int lanes, F join)
