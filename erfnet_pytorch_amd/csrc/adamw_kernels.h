@@ -15,26 +15,42 @@
 // A wave takes 256 consecutive elements at a time, four a lane: one 16-byte access of fp32, and exactly one scale.
 #pragma once
 #include "vec16.h"
+#include "wave.h"
 
-#define ADAMW_MAX_TENSORS 56
 #define ADAMW_BLOCK 256
 #define ADAMW_SCALE_BLOCK 256
 #define ADAMW_ROUNDS 4
 #define ADAMW_CHUNK (ADAMW_BLOCK * 4 * ADAMW_ROUNDS)
 #define ADAMW_TINY 7.8886090522101181e-31f      // 2^-100: 448 / x stays finite above it; blocks below are stored as zeros
 
-struct AdamwDesc {
-    void *p[ADAMW_MAX_TENSORS];
-    const void *g[ADAMW_MAX_TENSORS];
-    void *m[ADAMW_MAX_TENSORS], *v[ADAMW_MAX_TENSORS];          // BITS = 8: codes of m and of r
-    float *ms[ADAMW_MAX_TENSORS], *rs[ADAMW_MAX_TENSORS];       // BITS = 8: scales
-    long long n[ADAMW_MAX_TENSORS];
-    unsigned end_chunk[ADAMW_MAX_TENSORS];      // running total of chunks up to and including tensor i
-    int count;
+struct AdamwScalars {
     float b1, ob1, b2, ob2, keep, step, root_c2, eps;           // ob = 1 - b, keep = 1 - lr wd, step = lr / c1
 };
+// The pointers of one launch's tensors, as many as 4 KB of kernel arguments hold.
+template <int BITS> struct AdamwDesc {
+    static constexpr int MAX = 90;
+    AdamwScalars k;
+    int count;
+    unsigned end_chunk[MAX];    // running total of chunks up to and including tensor i
+    long long n[MAX];
+    void *p[MAX];
+    const void *g[MAX];
+    float *m[MAX], *v[MAX];
+};
+template <> struct AdamwDesc<8> {
+    static constexpr int MAX = 66;
+    AdamwScalars k;
+    int count;
+    unsigned end_chunk[MAX];
+    long long n[MAX];
+    void *p[MAX];
+    const void *g[MAX];
+    void *m[MAX], *r[MAX];      // codes of m and of the root
+    float *ms[MAX], *rs[MAX];   // their scales
+};
+static_assert(sizeof(AdamwDesc<32>) <= 4096 && sizeof(AdamwDesc<8>) <= 4096, "kernel arguments");
 
-__device__ __forceinline__ float adamw_update(const AdamwDesc &d, float p, float g, float &m, float &v, float &root)
+__device__ __forceinline__ float adamw_update(const AdamwScalars &d, float p, float g, float &m, float &v, float &root)
 {
     m = d.b1 * m + d.ob1 * g;
     v = d.b2 * v + d.ob2 * (g * g);
@@ -114,7 +130,7 @@ struct AdamwCodes {
             const float a = fabsf(x[j]);
             top = fmaxf(top, a < INFINITY ? a : 0.0f);
         }
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        top = wave_max(top);
         const bool some = top >= ADAMW_TINY;
         const float inv = some ? 448.0f / top : 0.0f;
         scale = some ? top / 448.0f : 0.0f;
@@ -131,49 +147,73 @@ struct AdamwCodes {
     }
 };
 
-template <typename T, int BITS>
-__global__ __launch_bounds__(ADAMW_BLOCK) void adamw_kernel(const AdamwDesc d)
+// A wave's `ADAMW_ROUNDS` blocks of 256 elements, the first at `base`, blocks ADAMW_BLOCK * 4 elements apart; all loads go
+// out before the first result is needed.  FULL: every element is there.
+template <typename T, int BITS, bool FULL>
+__device__ __forceinline__ void adamw_chunk(const AdamwDesc<BITS> &d, int t, long long n, long long base)
 {
-    // the tensor of this chunk: the number of running totals that are not above it (64 lanes look at all of them)
     const int lane = threadIdx.x & 63;
-    const bool past = lane < d.count && blockIdx.x >= d.end_chunk[lane < d.count ? lane : 0];
-    const int t = __popcll(__ballot(past));
-    const unsigned first = t ? d.end_chunk[t - 1] : 0u;
-    const long long n = d.n[t];
-    const long long base = (long long)(blockIdx.x - first) * ADAMW_CHUNK + (threadIdx.x >> 6) * ADAMW_SCALE_BLOCK;
+    f32x4 p[ADAMW_ROUNDS], g[ADAMW_ROUNDS], m[ADAMW_ROUNDS], v[ADAMW_ROUNDS];
+    unsigned cm[ADAMW_ROUNDS], cr[ADAMW_ROUNDS];
+    float ms[ADAMW_ROUNDS], rs[ADAMW_ROUNDS];
 #pragma unroll
     for (int r = 0; r < ADAMW_ROUNDS; ++r) {
-        const long long at = base + (long long)r * ADAMW_BLOCK * 4;       // this wave's 256 elements
-        if (at >= n) break;                                             // (uniform over the wave)
-        const long long i = at + lane * 4;
-        const int left = n - i >= 4 ? 4 : (int)(n - i);                 // may be negative
-        f32x4 p = AdamwQuad<T>::load(d.p[t], i, left);
-        const f32x4 g = AdamwQuad<T>::load(d.g[t], i, left);
-        f32x4 m, v, root;
-        if (BITS == 32) {
-            m = AdamwQuad<float>::load(d.m[t], i, left);
-            v = AdamwQuad<float>::load(d.v[t], i, left);
+        const long long at = base + (long long)r * ADAMW_BLOCK * 4, i = at + lane * 4;
+        const int left = FULL ? 4 : n - i >= 4 ? 4 : n - i > 0 ? (int)(n - i) : 0;
+        p[r] = AdamwQuad<T>::load(d.p[t], i, left);
+        g[r] = AdamwQuad<T>::load(d.g[t], i, left);
+        if constexpr (BITS == 32) {
+            m[r] = AdamwQuad<float>::load(d.m[t], i, left);
+            v[r] = AdamwQuad<float>::load(d.v[t], i, left);
         } else {
-            m = AdamwCodes::decode(AdamwCodes::load(d.m[t], i, left), d.ms[t][at / ADAMW_SCALE_BLOCK]);
-            v = AdamwCodes::decode(AdamwCodes::load(d.v[t], i, left), d.rs[t][at / ADAMW_SCALE_BLOCK]);
-            v *= v;
+            cm[r] = AdamwCodes::load(d.m[t], i, left);
+            cr[r] = AdamwCodes::load(d.r[t], i, left);
+            const bool there = FULL || at < n;
+            ms[r] = there ? d.ms[t][at / ADAMW_SCALE_BLOCK] : 0.0f;
+            rs[r] = there ? d.rs[t][at / ADAMW_SCALE_BLOCK] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < ADAMW_ROUNDS; ++r) {
+        const long long at = base + (long long)r * ADAMW_BLOCK * 4, i = at + lane * 4;
+        const int left = FULL ? 4 : n - i >= 4 ? 4 : n - i > 0 ? (int)(n - i) : 0;
+        if (!FULL && at >= n) break;            // (uniform over the wave)
+        f32x4 root;
+        if constexpr (BITS == 8) {
+            m[r] = AdamwCodes::decode(cm[r], ms[r]);
+            v[r] = AdamwCodes::decode(cr[r], rs[r]);
+            v[r] *= v[r];
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float mj = m[j], vj = v[j], rj;
-            p[j] = adamw_update(d, p[j], g[j], mj, vj, rj);
-            m[j] = mj; v[j] = vj; root[j] = rj;
+            float mj = m[r][j], vj = v[r][j], rj;
+            p[r][j] = adamw_update(d.k, p[r][j], g[r][j], mj, vj, rj);
+            m[r][j] = mj; v[r][j] = vj; root[j] = rj;
         }
-        AdamwQuad<T>::store(d.p[t], i, left, p);
-        if (BITS == 32) {
-            AdamwQuad<float>::store(d.m[t], i, left, m);
-            AdamwQuad<float>::store(d.v[t], i, left, v);
+        AdamwQuad<T>::store(d.p[t], i, left, p[r]);
+        if constexpr (BITS == 32) {
+            AdamwQuad<float>::store(d.m[t], i, left, m[r]);
+            AdamwQuad<float>::store(d.v[t], i, left, v[r]);
         } else {
-            float ms, rs;
-            const unsigned cm = AdamwCodes::encode<false>(m, ms), cr = AdamwCodes::encode<true>(root, rs);
-            AdamwCodes::store(d.m[t], i, left, cm);
-            AdamwCodes::store(d.v[t], i, left, cr);
-            if (lane == 0) { d.ms[t][at / ADAMW_SCALE_BLOCK] = ms; d.rs[t][at / ADAMW_SCALE_BLOCK] = rs; }
+            float sm, sr;
+            const unsigned nm = AdamwCodes::encode<false>(m[r], sm), nr = AdamwCodes::encode<true>(root, sr);
+            AdamwCodes::store(d.m[t], i, left, nm);
+            AdamwCodes::store(d.r[t], i, left, nr);
+            if (lane == 0) { d.ms[t][at / ADAMW_SCALE_BLOCK] = sm; d.rs[t][at / ADAMW_SCALE_BLOCK] = sr; }
         }
     }
+}
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(ADAMW_BLOCK) void adamw_kernel(const AdamwDesc<BITS> d)
+{
+    // the tensor of this chunk: the number of running totals that are not above it (64 lanes look at two each)
+    const int lane = threadIdx.x & 63, l0 = lane < d.count ? lane : 0, l1 = lane + 64 < d.count ? lane + 64 : 0;
+    const int t = __popcll(__ballot(lane < d.count && blockIdx.x >= d.end_chunk[l0])) +
+                  __popcll(__ballot(lane + 64 < d.count && blockIdx.x >= d.end_chunk[l1]));
+    const unsigned first = t ? d.end_chunk[t - 1] : 0u;
+    const long long n = d.n[t], chunk = (long long)(blockIdx.x - first) * ADAMW_CHUNK;
+    const long long base = chunk + (threadIdx.x >> 6) * ADAMW_SCALE_BLOCK;
+    if (chunk + ADAMW_CHUNK <= n) adamw_chunk<T, BITS, true>(d, t, n, base);
+    else adamw_chunk<T, BITS, false>(d, t, n, base);
 }

@@ -263,14 +263,14 @@ int adamw_step(const char *what, int count, void *const *p, const void *const *g
     if (!(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0)) return fail("%s: betas outside [0, 1)", what);
     if (!(eps >= 0.0) || !(lr >= 0.0) || !(wd >= 0.0)) return fail("%s: negative lr / eps / weight decay", what);
     if (count && (!p || !g || !m || !v || !numel || (BITS == 8 && (!ms || !vs)))) return fail("%s: null pointer table", what);
-    AdamwDesc d;
+    AdamwDesc<BITS> d;
     memset(&d, 0, sizeof(d));
     // the scalars in double, rounded once for the kernel
-    d.b1 = (float)b1; d.ob1 = (float)(1.0 - b1); d.b2 = (float)b2; d.ob2 = (float)(1.0 - b2);
-    d.keep = (float)(1.0 - lr * wd);
-    d.step = (float)(lr / (1.0 - pow(b1, (double)step)));
-    d.root_c2 = (float)sqrt(1.0 - pow(b2, (double)step));
-    d.eps = (float)eps;
+    d.k.b1 = (float)b1; d.k.ob1 = (float)(1.0 - b1); d.k.b2 = (float)b2; d.k.ob2 = (float)(1.0 - b2);
+    d.k.keep = (float)(1.0 - lr * wd);
+    d.k.step = (float)(lr / (1.0 - pow(b1, (double)step)));
+    d.k.root_c2 = (float)sqrt(1.0 - pow(b2, (double)step));
+    d.k.eps = (float)eps;
     for (int i = 0; i < count; ++i) {
         if (numel[i] < 0) return fail("%s: tensor %d has a negative size", what, i);
         if (numel[i] && (!p[i] || !g[i] || !m[i] || !v[i] || (BITS == 8 && (!ms[i] || !vs[i]))))
@@ -281,14 +281,14 @@ int adamw_step(const char *what, int count, void *const *p, const void *const *g
     while (i < count) {
         d.count = 0;
         unsigned long long chunks = 0;
-        for (; i < count && d.count < ADAMW_MAX_TENSORS; ++i) {
+        for (; i < count && d.count < AdamwDesc<BITS>::MAX; ++i) {
             if (numel[i] == 0) continue;
             const unsigned long long c = ((unsigned long long)numel[i] + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
             if (chunks + c >= (1ull << 31)) break;              // goes into the next launch
             const int k = d.count++;
-            d.p[k] = p[i]; d.g[k] = g[i]; d.m[k] = m[i]; d.v[k] = v[i];
-            d.ms[k] = BITS == 8 ? ms[i] : nullptr;
-            d.rs[k] = BITS == 8 ? vs[i] : nullptr;
+            d.p[k] = p[i]; d.g[k] = g[i];
+            if constexpr (BITS == 8) { d.m[k] = m[i]; d.r[k] = v[i]; d.ms[k] = ms[i]; d.rs[k] = vs[i]; }
+            else { d.m[k] = (float *)m[i]; d.v[k] = (float *)v[i]; }
             d.n[k] = numel[i];
             chunks += c;
             d.end_chunk[k] = (unsigned)chunks;
