@@ -7,6 +7,7 @@ every GPU call raises, there is no fallback.  ``build()`` compiles it in-tree wi
 import ctypes as C
 import os
 import subprocess
+import sysconfig
 import threading
 
 # torch must come first: it brings the HIP runtime (its bundled libamdhip64) that owns the tensors'
@@ -49,26 +50,54 @@ DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 TRANSLATION_UNITS = ("erfnet_hip.hip", "train_ops.hip")
+_HOST_SRC = os.path.join(_SRC, "host_ext.cpp")
+_HOST_SO = os.path.join(_HERE, "_host.so")
+_host = None
 
 
 def sources():
-    return [os.path.join(_SRC, f) for f in sorted(os.listdir(_SRC))] + \
+    return [os.path.join(_SRC, f) for f in sorted(os.listdir(_SRC)) if f != "host_ext.cpp"] + \
         [os.path.join(os.path.dirname(_HERE), "include", "erfnet_hip.h")]
 
 
+def _run(cmd, verbose):
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.check_call(cmd)
+
+
 def build(force=False, verbose=False):
-    """Compile csrc/*.hip -> liberfnet_hip.so for gfx950 if it is missing or stale."""
+    """Compile csrc/*.hip -> liberfnet_hip.so for gfx950, and csrc/host_ext.cpp -> _host.so (the host side of an
+    optimiser step, against torch's C++ headers), whichever is missing or stale."""
+    if force or not os.path.exists(_HOST_SO) or os.path.getmtime(_HOST_SO) < os.path.getmtime(_HOST_SRC):
+        base = os.path.dirname(torch.__file__)
+        inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"]]
+        lib_dir = os.path.join(base, "lib")
+        _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", *("-I" + i for i in inc),
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", _HOST_SRC, "-o", _HOST_SO, "-L" + lib_dir,
+              "-lc10", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath," + lib_dir], verbose)
     srcs = sources()
     if not force and os.path.exists(_SO) and \
             os.path.getmtime(_SO) >= max(os.path.getmtime(s) for s in srcs):
         return _SO
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", *DEVICE_FLAGS,
-           "-o", _SO, *(os.path.join(_SRC, f) for f in TRANSLATION_UNITS)]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd)
+    _run([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", *DEVICE_FLAGS,
+          "-o", _SO, *(os.path.join(_SRC, f) for f in TRANSLATION_UNITS)], verbose)
     return _SO
+
+
+def host():
+    """The C++ host module; raises RuntimeError (there is no Python stand-in) when it is not built."""
+    global _host
+    if _host is None:
+        try:
+            from . import _host as module
+        except ImportError as e:
+            raise RuntimeError(f"cannot load {_HOST_SO}: {e}; build it with `python -c 'import __graft_entry__ as g; "
+                               "g.build()'`") from e
+        _host = module
+    return _host
 
 
 _PROTOS = {

@@ -277,6 +277,13 @@ int adamw_step(const char *what, int count, void *const *p, const void *const *g
             return fail("%s: tensor %d has a null pointer", what, i);
         if (numel[i] / ADAMW_CHUNK >= (1ll << 31) - 1) return fail("%s: tensor %d is too large", what, i);
     }
+    // a replayed launch would repeat this step's bias corrections
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (std::any_of(numel, numel + count, [](long long n) { return n > 0; }) &&
+        (hipStreamIsCapturing(st, &capture) != hipSuccess || capture != hipStreamCaptureStatusNone)) {
+        (void)hipGetLastError();
+        return fail("%s: the step cannot be captured into a graph", what);
+    }
     int i = 0;
     while (i < count) {
         d.count = 0;

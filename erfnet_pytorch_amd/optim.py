@@ -40,13 +40,12 @@ class _Tables:
         return self.ptrs, self.numel
 
 
-def _usable(p, what, dtypes=(torch.float32,)):
+def _usable(p, what):
     if not p.is_cuda:
         raise RuntimeError(f"erfnet_pytorch_amd.optim: {what} lives on {p.device}; the update kernels "
                            "run on the GPU only (use torch.optim for host tensors)")
-    if p.dtype not in dtypes:
-        raise TypeError(f"erfnet_pytorch_amd.optim: {what} is {p.dtype}; parameters and gradients are " +
-                        ("fp32" if dtypes == (torch.float32,) else "fp32 or bf16, one type for both"))
+    if p.dtype != torch.float32:
+        raise TypeError(f"erfnet_pytorch_amd.optim: {what} is {p.dtype}; parameters and gradients are fp32")
     if not p.is_contiguous():
         raise ValueError(f"erfnet_pytorch_amd.optim: {what} is not contiguous")
 
@@ -159,7 +158,8 @@ class SGD(torch.optim.Optimizer):
 
 
 class AdamW(torch.optim.Optimizer):
-    """``torch.optim.AdamW`` (no amsgrad, no maximize) for fp32 and bf16 parameters, one launch per 56 tensors.
+    """``torch.optim.AdamW`` (no amsgrad, no maximize) for fp32 and bf16 parameters, one launch per 90 tensors (66 with
+    8-bit moments).
 
     ``state_bits=32``: fp32 moments under torch's key names, so that state dicts travel between the two classes.
     ``state_bits=8``: both moments as float8 (e4m3) with one fp32 scale per 256 consecutive elements — ``exp_avg``,
@@ -167,7 +167,9 @@ class AdamW(torch.optim.Optimizer):
     code * scale): 2 bytes an element held instead of 8.  The update itself uses the moments before they are
     rounded.  ``load_state_dict`` takes the state of an optimiser with the same ``state_bits`` only.
 
-    ``step`` cannot be captured into a HIP graph: the bias corrections of the step go into the launch."""
+    ``step`` cannot be captured into a HIP graph (the library refuses): the bias corrections go into the launch."""
+
+    _entry_points = None
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
         if lr < 0.0 or eps < 0.0 or weight_decay < 0.0:
@@ -176,11 +178,14 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: betas {betas} outside [0, 1)")
         if state_bits not in (8, 32):
             raise ValueError(f"AdamW: state_bits must be 8 or 32 (got {state_bits})")
-        self.state_bits = state_bits
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False,
                                       maximize=False, foreach=None, capturable=False, differentiable=False,
                                       fused=None, decoupled_weight_decay=True))
-        self._tables = {}
+        self.defaults["state_bits"] = state_bits        # (what a copied or unpickled optimiser keeps)
+
+    @property
+    def state_bits(self):
+        return self.defaults["state_bits"]
 
     @property
     def _moments(self):
@@ -189,11 +194,12 @@ class AdamW(torch.optim.Optimizer):
             ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale")
 
     def _new_state(self, p):
+        new = {"step": torch.tensor(0.0)}
         if self.state_bits == 32:
-            return {k: torch.zeros_like(p, dtype=torch.float32) for k in self._moments}
+            return new | {k: torch.zeros_like(p, dtype=torch.float32) for k in self._moments}
         scales = -(-p.numel() // 256)
-        return {k: torch.zeros(scales, dtype=torch.float32, device=p.device) if k.endswith("_scale") else
-                torch.zeros_like(p, dtype=torch.float8_e4m3fn) for k in self._moments}
+        return new | {k: torch.zeros(scales, dtype=torch.float32, device=p.device) if k.endswith("_scale") else
+                      torch.zeros_like(p, dtype=torch.float8_e4m3fn) for k in self._moments}
 
     def load_state_dict(self, state_dict):
         want = set(self._moments)
@@ -205,8 +211,11 @@ class AdamW(torch.optim.Optimizer):
         # torch casts floating-point state to the parameter's type; the moments keep their own
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
-            for k in want if i in state_dict["state"] else ():
-                self.state[p][k] = state_dict["state"][i][k].detach().to(p.device, copy=True)
+            if i in state_dict["state"]:
+                given = state_dict["state"][i]
+                for k in want:
+                    self.state[p][k] = given[k].detach().to(p.device, copy=True).contiguous()
+                self.state[p]["step"] = torch.tensor(float(given["step"]))
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -214,39 +223,24 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        lib = _lib.lib()
-        for gi, group in enumerate(self.param_groups):
+        host, fns = _lib.host(), self._entry_points
+        if fns is None:
+            lib, name = _lib.lib(), "erf_adamw_step" if self.state_bits == 32 else "erf_adamw8_step"
+            fns = self._entry_points = tuple(C.cast(getattr(lib, name + s), C.c_void_p).value for s in ("", "_bf16"))
+        for group in self.param_groups:
             if group.get("amsgrad") or group.get("maximize") or not group.get("decoupled_weight_decay", True):
                 raise NotImplementedError("erfnet_pytorch_amd.optim.AdamW: amsgrad / maximize / L2 weight decay are "
                                           "not implemented (Adam has the latter)")
-            lists = {}
-            for p in group["params"]:
-                g = p.grad
-                if g is None:
-                    continue
-                if g.is_sparse:
-                    raise RuntimeError("erfnet_pytorch_amd.optim: sparse gradients are not supported")
-                _usable(p, "a parameter", (torch.float32, torch.bfloat16))
-                _usable(g, "a gradient", (p.dtype,))
-                st = self.state[p]
-                if not st:
-                    st["step"] = torch.tensor(0.0)
-                    st.update(self._new_state(p))
-                lists.setdefault((p.device, p.dtype, int(st["step"])), []).append((p, g, st))
-            for li, ((dev, dtype, step), items) in enumerate(lists.items()):
-                with torch.cuda.device(dev):
-                    if torch.cuda.is_current_stream_capturing():
-                        raise RuntimeError("erfnet_pytorch_amd.optim.AdamW: step() cannot be captured into a graph")
-                    tensors = [[p for p, _, _ in items], [g for _, g, _ in items]]
-                    tensors += [[st[k] for _, _, st in items] for k in self._moments]
-                    tab = self._tables.setdefault((gi, li), _Tables(len(tensors)))
-                    ptrs, numel = tab.update(tensors)
-                    fn = getattr(lib, ("erf_adamw_step" if self.state_bits == 32 else "erf_adamw8_step") +
-                                 ("_bf16" if dtype == torch.bfloat16 else ""))
-                    b1, b2 = group["betas"]
-                    _lib.check(fn(len(items), *ptrs, numel, float(group["lr"]), float(b1), float(b2),
-                                  float(group["eps"]), float(group["weight_decay"]), step + 1,
-                                  C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)))
-                for _, _, st in items:
-                    st["step"] = torch.tensor(float(step + 1))
+            b1, b2 = group["betas"]
+            args = (group["params"], self.state, self._moments, self.state_bits, *fns, float(group["lr"]), float(b1),
+                    float(b2), float(group["eps"]), float(group["weight_decay"]), torch._C._cuda_getCurrentRawStream)
+            left = host.adamw_step(*args)
+            if left:                    # parameters that have their first gradient
+                if isinstance(left, int):
+                    _lib.check(left)
+                for p in left:
+                    self.state[p].update(self._new_state(p))
+                left = host.adamw_step(*args)
+                if left:
+                    _lib.check(left)
         return loss

@@ -640,6 +640,81 @@ def test_adamw_views_at_odd_offsets():
         assert torch.equal(p, q) and torch.equal(base[:3], keep[:3]) and torch.equal(base[1003:], keep[1003:])
 
 
+@gpu
+def test_adamw_moves_the_version_of_what_it_updates():
+    """Copies kept of a parameter go by its version: a bf16 parameter's fp32 copy is fresh after a step."""
+    from erfnet_pytorch_amd import functional as hipf, optim
+    w = torch.nn.Parameter(torch.ones(64, dtype=torch.bfloat16, device=DEV))
+    x = torch.randn(8, 64, generator=torch.Generator().manual_seed(0)).to(DEV)
+    first = hipf.layer_norm(x, w).detach()
+    opt = optim.AdamW([w], lr=0.5, weight_decay=0.0)
+    w.grad = torch.ones_like(w)
+    before = w._version
+    opt.step()
+    assert w._version > before
+    assert torch.equal(w.detach().float(), torch.full((64,), 0.5, device=DEV))
+    assert torch.equal(hipf.layer_norm(x, w).detach(), first * 0.5)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_copies_and_refuses_capture(bits):
+    import copy
+    from erfnet_pytorch_amd import optim
+    p = torch.nn.Parameter(torch.ones(300, device=DEV))
+    opt = optim.AdamW([p], state_bits=bits)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    twin = copy.deepcopy(opt)
+    q = twin.param_groups[0]["params"][0]
+    q.grad = torch.ones_like(q)
+    opt.step(), twin.step()
+    assert twin.state_bits == bits and torch.equal(p, q)
+    kept = p.detach().clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()
+        mark = kept * 2
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(p.detach(), kept) and torch.equal(mark, kept * 2) and float(opt.state[p]["step"]) == 2
+
+
+@gpu
+def test_adamw_refuses_state_and_gradients_that_do_not_fit():
+    from erfnet_pytorch_amd import optim
+    p = torch.nn.Parameter(torch.ones(300, device=DEV))
+    opt = optim.AdamW([p], state_bits=8)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    kept = p.detach().clone()
+    st = opt.state[p]
+    for key, bad, error in (("exp_avg_scale", torch.zeros(1, device=DEV), ValueError),
+                            ("exp_avg", torch.zeros(300, device=DEV), ValueError),
+                            ("exp_avg_sq_root", torch.zeros(300, dtype=torch.float8_e4m3fn), RuntimeError),
+                            ("step", torch.zeros(1, device=DEV), ValueError)):
+        good, st[key] = st[key], bad
+        with pytest.raises(error):
+            opt.step()
+        st[key] = good
+    st.pop("exp_avg")
+    with pytest.raises(KeyError):
+        opt.step()
+    wide = torch.zeros(300, 2, device=DEV)
+    q = torch.nn.Parameter(wide[:, 0])
+    q.grad = torch.ones(300, device=DEV)
+    with pytest.raises(ValueError, match="contiguous"):
+        optim.AdamW([q]).step()
+    h = torch.nn.Parameter(torch.ones(4, device=DEV, dtype=torch.float16))
+    h.grad = torch.ones_like(h)
+    with pytest.raises(TypeError):
+        optim.AdamW([h]).step()
+    torch.cuda.synchronize()
+    assert torch.equal(p.detach(), kept)
+
+
 # ================================================================================ together, streams, graphs
 def head_step(hipf, x, w, b, lin, t):
     """Norm, a linear head, log probabilities and an entropy bonus: the loss of one step."""
