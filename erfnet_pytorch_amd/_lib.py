@@ -5,6 +5,7 @@ every GPU call raises, there is no fallback.  ``build()`` compiles it in-tree wi
 (cross-compiles without a GPU).
 """
 import ctypes as C
+import importlib
 import os
 import subprocess
 import sysconfig
@@ -52,7 +53,7 @@ DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 TRANSLATION_UNITS = ("erfnet_hip.hip", "train_ops.hip")
 _HOST_SRC = os.path.join(_SRC, "host_ext.cpp")
 _HOST_SO = os.path.join(_HERE, "_host.so")
-_host = None
+_host_module = None
 
 
 def sources():
@@ -67,16 +68,18 @@ def _run(cmd, verbose):
 
 
 def build(force=False, verbose=False):
-    """Compile csrc/*.hip -> liberfnet_hip.so for gfx950, and csrc/host_ext.cpp -> _host.so (the host side of an
-    optimiser step, against torch's C++ headers), whichever is missing or stale."""
-    if force or not os.path.exists(_HOST_SO) or os.path.getmtime(_HOST_SO) < os.path.getmtime(_HOST_SRC):
+    """Compile csrc/*.hip -> liberfnet_hip.so for gfx950, and csrc/host_ext.cpp -> _host.so (the host side of short
+    calls, against torch's C++ headers), whichever is missing or stale."""
+    header = os.path.join(os.path.dirname(_HERE), "include", "erfnet_hip.h")
+    if force or not os.path.exists(_HOST_SO) or \
+            os.path.getmtime(_HOST_SO) < max(os.path.getmtime(_HOST_SRC), os.path.getmtime(header)):
         base = os.path.dirname(torch.__file__)
         inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
-               sysconfig.get_paths()["include"]]
+               sysconfig.get_paths()["include"], os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")]
         lib_dir = os.path.join(base, "lib")
         _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", *("-I" + i for i in inc),
-              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", _HOST_SRC, "-o", _HOST_SO, "-L" + lib_dir,
-              "-lc10", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath," + lib_dir], verbose)
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__", _HOST_SRC, "-o", _HOST_SO, "-L" + lib_dir,
+              "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath," + lib_dir], verbose)
     srcs = sources()
     if not force and os.path.exists(_SO) and \
             os.path.getmtime(_SO) >= max(os.path.getmtime(s) for s in srcs):
@@ -89,15 +92,17 @@ def build(force=False, verbose=False):
 
 def host():
     """The C++ host module; raises RuntimeError (there is no Python stand-in) when it is not built."""
-    global _host
-    if _host is None:
+    global _host_module
+    if _host_module is None:
+        handle = lib()
         try:
-            from . import _host as module
+            module = importlib.import_module(__package__ + "._host")
         except ImportError as e:
             raise RuntimeError(f"cannot load {_HOST_SO}: {e}; build it with `python -c 'import __graft_entry__ as g; "
                                "g.build()'`") from e
-        _host = module
-    return _host
+        module.bind(lambda name: C.cast(getattr(handle, name), C.c_void_p).value)
+        _host_module = module
+    return _host_module
 
 
 _PROTOS = {

@@ -1,30 +1,293 @@
-// erfnet_pytorch_amd._host: the part of an optimiser step that looks at every parameter, in C++.
-//
-// A step over the 229 parameter tensors of the 20-class network is 20 us of GPU work; gathering their pointers
-// through Python attributes took 560 us.  Nothing is kept between calls: every step reads the gradients,
-// the state tensors and their pointers anew.
+// erfnet_pytorch_amd._host: the host side of the calls that are shorter than their Python would be.
+//   layer_norm, log_probs: autograd nodes over the C ABI (a backward pass that enters Python from autograd's thread took
+//     twice the time of the kernels it launched: 110 us for a layer norm of 256 x 128, forward and backward);
+//   adamw_step: one pass over the parameters (229 of them: 20 us of GPU work, 560 us of Python attributes).
+// Arguments come checked from functional.py / optim.py.  Nothing is kept between calls.
 #include <Python.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <optional>
+#include <stdexcept>
+#include <string>
 #include <vector>
+
+#include "../../include/erfnet_hip.h"
 
 namespace {
 
-typedef int (*adamw32_fn)(int, void *const *, const void *const *, void *const *, void *const *, const long long *, double,
-                          double, double, double, double, long long, void *);
-typedef int (*adamw8_fn)(int, void *const *, const void *const *, void *const *, void *const *, void *const *, void *const *,
-                         const long long *, double, double, double, double, double, long long, void *);
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
+// The library's entry points for fp32 and bf16 tensors, handed over once by bind() (the library that the package has loaded,
+// wherever it lies).
+struct Library {
+    decltype(&erf_last_error) last_error;
+    decltype(&erf_layer_norm_workspace_bytes) norm_ws;
+    decltype(&erf_log_probs_workspace_bytes) logp_ws;
+    decltype(&erf_layer_norm_forward_bf16) norm_fwd[2];
+    decltype(&erf_layer_norm_backward_bf16) norm_bwd[2];
+    decltype(&erf_log_probs_forward_bf16) logp_fwd[2];
+    decltype(&erf_log_probs_backward_bf16) logp_bwd[2];
+    decltype(&erf_adamw_step_bf16) adamw[2];
+    decltype(&erf_adamw8_step_bf16) adamw8[2];
+} lib;
+
+int kind(const Tensor &t) { return t.scalar_type() == at::kBFloat16; }
+void check(int rc)
+{
+    if (rc) throw std::runtime_error(std::string("erfnet_hip: ") + lib.last_error());
+}
+void *stream(const c10::Device &d) { return c10::hip::getCurrentHIPStream(d.index()).stream(); }
+float *floats(const Tensor &t) { return t.defined() ? (float *)t.data_ptr() : nullptr; }
+Tensor parameter(const Tensor &t) { return t.defined() ? t.to(at::kFloat).contiguous() : t; }
+
+// What backward returns, from an operator whose gradient has none: where a graph of the backward pass is recorded
+// (`recorded`), the results hang on a node that raises, in front of everything that they depend on.
+variable_list first_order(variable_list grads, bool recorded, const variable_list &inputs)
+{
+    if (!recorded) return grads;
+    bool any = false;
+    for (const Tensor &t : inputs) any |= t.defined() && t.requires_grad();
+    if (!any) return grads;
+    const at::AutoGradMode on(true);
+    auto node = std::make_shared<torch::autograd::Error>(
+        "erfnet_pytorch_amd: the gradient of layer_norm / log_probs is not differentiable",
+        torch::autograd::collect_next_edges(inputs));
+    for (Tensor &g : grads)
+        if (g.defined()) torch::autograd::set_history(g, node);
+    return grads;
+}
+
+// ---------------------------------------------------------------------------------------------- layer norm
+// Rows of C contiguous channels: the last axis as it is, axis 1 of an image as NHWC memory.
+Tensor norm_rows(const Tensor &x, bool image)
+{
+    return image ? x.contiguous(at::MemoryFormat::ChannelsLast) : x.contiguous();
+}
+
+Tensor norm_forward(const Tensor &x, const Tensor &w, const Tensor &b, double eps, bool image, Tensor *stat)
+{
+    const int64_t c = x.size(image ? 1 : -1), rows = x.numel() / c;
+    const c10::DeviceGuard guard(x.device());
+    const Tensor wf = parameter(w), bf = parameter(b);
+    Tensor y = at::empty_like(x);
+    if (stat) *stat = at::empty({2, rows}, x.options().dtype(at::kFloat));
+    float *kept = stat ? floats(*stat) : nullptr;
+    check(lib.norm_fwd[kind(x)](x.data_ptr(), floats(wf), floats(bf), y.data_ptr(), kept, kept ? kept + rows : nullptr, rows,
+                                (int)c, (float)eps, stream(x.device())));
+    return y;
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x0, const std::optional<Tensor> &w0, const std::optional<Tensor> &b0,
+                          double eps, bool image)
+    {
+        const Tensor x = norm_rows(x0, image), w = w0.value_or(Tensor()), b = b0.value_or(Tensor());
+        Tensor stat;
+        Tensor y = norm_forward(x, w, b, eps, image, &stat);
+        ctx->save_for_backward({x, w, stat});
+        ctx->saved_data["image"] = image;
+        ctx->saved_data["bias"] = b.defined() ? (int64_t)b.scalar_type() : (int64_t)-1;
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &stat = saved[2];
+        const bool image = ctx->saved_data["image"].toBool();
+        const int64_t bias = ctx->saved_data["bias"].toInt();
+        const int64_t c = x.size(image ? 1 : -1), rows = stat.size(1);
+        const c10::DeviceGuard guard(x.device());
+        const bool recorded = at::GradMode::is_enabled();
+        const at::AutoGradMode off(false);
+        const Tensor gy = norm_rows(grads[0].to(x.scalar_type()), image), wf = parameter(w);
+        Tensor dx, dw, db, ws;
+        if (ctx->needs_input_grad(0)) dx = at::empty_like(x);
+        const auto f32 = x.options().dtype(at::kFloat);
+        // (an absent weight has no edge)
+        if (w.defined() && ctx->needs_input_grad(1)) dw = at::empty({c}, f32);
+        if (bias >= 0 && ctx->needs_input_grad(w.defined() ? 2 : 1)) db = at::empty({c}, f32);
+        int64_t n_ws = 0;
+        if (dw.defined() || db.defined()) {
+            n_ws = (int64_t)lib.norm_ws(rows, (int)c);
+            ws = at::empty({n_ws}, x.options().dtype(at::kByte));
+        }
+        check(lib.norm_bwd[kind(x)](x.data_ptr(), floats(wf), floats(stat), floats(stat) + rows, gy.data_ptr(),
+                                    dx.defined() ? dx.data_ptr() : nullptr, floats(dw), floats(db), rows, (int)c,
+                                    ws.defined() ? ws.data_ptr() : nullptr, (size_t)n_ws, stream(x.device())));
+        if (dw.defined()) dw = dw.to(w.scalar_type());
+        if (db.defined()) db = db.to((at::ScalarType)bias);
+        return first_order({dx, dw, db, Tensor(), Tensor()}, recorded, {x, w, grads[0]});
+    }
+};
+
+// ---------------------------------------------------------------------------------------------- log probabilities
+struct LogpShape {
+    int64_t outer, v, inner, ld, top_k, ignore, axis;
+    bool moved;                     // the class axis was brought to the end
+};
+
+// The results in the caller's shapes; what backward needs goes to kept: the logits as the kernels read them, the targets,
+// the statistics, the entropy and the alternatives' indices as the kernels wrote them.
+variable_list logp_forward(const Tensor &logits, const Tensor &target0, LogpShape &s, variable_list &kept)
+{
+    const int64_t nd = logits.dim();
+    s.v = logits.size(s.axis);
+    s.inner = 1;
+    for (int64_t i = s.axis + 1; i < nd; ++i) s.inner *= logits.size(i);
+    Tensor x;
+    const Tensor target = target0.contiguous();
+    const int64_t pixels = target.numel();
+    const c10::DeviceGuard guard(logits.device());
+    std::vector<int64_t> full;
+    // The pixel kernel gives a thread a pixel; it needs enough of them to fill the card, and keeps up to 8
+    // alternatives in registers.
+    const bool plane = s.inner > 1 && s.v <= 256 && s.top_k <= ERF_LOG_PROBS_MAX_TOP_PIXELS && pixels >= 4096;
+    s.moved = !plane && s.axis != nd - 1;
+    if (plane) {
+        x = logits.contiguous();
+        s.outer = pixels / s.inner;
+        s.ld = 0;
+    } else {
+        x = (s.moved ? logits.movedim(s.axis, -1) : logits).reshape({pixels, s.v});
+        s.outer = pixels;
+        s.inner = 1;
+        if (x.stride(1) != 1 || (pixels > 1 && x.stride(0) < s.v)) x = x.contiguous();
+        s.ld = pixels > 1 ? x.stride(0) : s.v;
+    }
+    for (int64_t i = 0; i < nd; ++i)
+        if (i != s.axis) full.push_back(logits.size(i));
+        else if (!s.moved) full.push_back(s.top_k);
+    if (s.moved) full.push_back(s.top_k);
+    const auto f32 = logits.options().dtype(at::kFloat);
+    const Tensor lp = at::empty(target.sizes(), f32), ent = at::empty(target.sizes(), f32), top = at::empty(full, f32);
+    const Tensor idx = at::empty(full, f32.dtype(at::kLong));
+    const Tensor stats = at::empty({2 * pixels}, f32);
+    Tensor ws;
+    const int64_t n_ws = (int64_t)lib.logp_ws(s.outer, (int)s.v, s.inner, (int)s.top_k);
+    if (n_ws) ws = at::empty({n_ws}, f32.dtype(at::kByte));
+    check(lib.logp_fwd[kind(x)](x.data_ptr(), (const long long *)target.data_ptr(), floats(lp), floats(ent), floats(stats), floats(top),
+                                (long long *)idx.data_ptr(), s.outer, (int)s.v, s.inner, s.ld, (int)s.top_k, s.ignore,
+                                ws.defined() ? ws.data_ptr() : nullptr, (size_t)n_ws, stream(x.device())));
+    kept = {x, target, stats, ent, idx};
+    if (s.moved) return {lp, ent, top.movedim(-1, s.axis), idx.movedim(-1, s.axis)};
+    return {lp, ent, top, idx};
+}
+
+struct LogProbs : torch::autograd::Function<LogProbs> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &target0, int64_t top_k,
+                                 int64_t ignore, int64_t axis)
+    {
+        LogpShape s{0, 0, 0, 0, top_k, ignore, axis, false};
+        variable_list kept, out = logp_forward(logits, target0, s, kept);
+        ctx->save_for_backward(kept);
+        ctx->saved_data["shape"] = std::vector<int64_t>{s.outer, s.v, s.inner, s.ld, s.top_k, s.ignore, s.axis, s.moved};
+        ctx->saved_data["logits"] = logits.sizes().vec();
+        ctx->mark_non_differentiable({out[3]});
+        ctx->set_materialize_grads(false);
+        return out;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &target = saved[1], &stats = saved[2], &ent = saved[3], &idx = saved[4];
+        const std::vector<int64_t> s = ctx->saved_data["shape"].toIntVector();
+        std::vector<int64_t> shape = ctx->saved_data["logits"].toIntVector();
+        const int64_t axis = s[6];
+        const bool moved = s[7] != 0;
+        const c10::DeviceGuard guard(x.device());
+        const bool recorded = at::GradMode::is_enabled();
+        const at::AutoGradMode off(false);
+        Tensor g[3];
+        for (int i = 0; i < 3; ++i)
+            if (grads[i].defined())
+                g[i] = (moved && i == 2 ? grads[i].movedim(axis, -1) : grads[i]).to(at::kFloat).contiguous();
+        if (moved) {
+            shape.push_back(shape[axis]);
+            shape.erase(shape.begin() + axis);
+        }
+        Tensor dx = at::empty(shape, x.options());
+        check(lib.logp_bwd[kind(x)](x.data_ptr(), (const long long *)target.data_ptr(), floats(ent), floats(stats),
+                                    (const long long *)idx.data_ptr(), floats(g[0]), floats(g[1]), floats(g[2]), dx.data_ptr(),
+                                    s[0], (int)s[1], s[2], s[3], (int)s[4], s[5], stream(x.device())));
+        if (moved) dx = dx.movedim(-1, axis);
+        return first_order({dx, Tensor(), Tensor(), Tensor(), Tensor()}, recorded, {x, grads[0], grads[1], grads[2]});
+    }
+};
+
+bool wanted(std::initializer_list<Tensor> inputs)
+{
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor &t : inputs)
+        if (t.defined() && t.requires_grad()) return true;
+    return false;
+}
+Tensor unpack(PyObject *o) { return o == Py_None ? Tensor() : THPVariable_Unpack(o); }
+
+// layer_norm(x, weight or None, bias or None, eps, image)
+PyObject *layer_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    if (nargs != 5 || !THPVariable_Check(args[0])) {
+        PyErr_SetString(PyExc_TypeError, "layer_norm: (tensor, weight, bias, eps, image)");
+        return nullptr;
+    }
+    const Tensor x = unpack(args[0]), w = unpack(args[1]), b = unpack(args[2]);
+    const double eps = PyFloat_AsDouble(args[3]);
+    const bool image = PyObject_IsTrue(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    auto given = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+    if (wanted({x, w, b})) return THPVariable_Wrap(LayerNorm::apply(x, given(w), given(b), eps, image));
+    return THPVariable_Wrap(norm_forward(norm_rows(x, image), w, b, eps, image, nullptr));
+    END_HANDLE_TH_ERRORS
+}
+
+// log_probs(logits, target, top_k, ignore_index, axis) -> (log_prob, entropy, top, indices)
+PyObject *log_probs(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    if (nargs != 5 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1])) {
+        PyErr_SetString(PyExc_TypeError, "log_probs: (tensor, tensor, top_k, ignore_index, axis)");
+        return nullptr;
+    }
+    const Tensor logits = unpack(args[0]), target = unpack(args[1]);
+    const int64_t top_k = PyLong_AsLongLong(args[2]), ignore = PyLong_AsLongLong(args[3]), axis = PyLong_AsLongLong(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    variable_list out;
+    if (wanted({logits})) {
+        out = LogProbs::apply(logits, target, top_k, ignore, axis);
+    } else {
+        LogpShape s{0, 0, 0, 0, top_k, ignore, axis, false};
+        variable_list kept;
+        out = logp_forward(logits, target, s, kept);
+    }
+    THPObjectPtr tuple(PyTuple_New(4));
+    if (!tuple) return nullptr;
+    for (int i = 0; i < 4; ++i) {
+        PyObject *o = THPVariable_Wrap(out[i]);
+        if (!o) return nullptr;
+        PyTuple_SET_ITEM(tuple.get(), i, o);
+    }
+    return tuple.release();
+    END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------------------------------------- AdamW
 struct Batch {                      // the tensors of one launch list: a device, a type and a step count
     c10::Device device;
     at::ScalarType type;
     long long step;
-    std::vector<void *> p, s[4];
+    std::vector<void *> p, s[4];        // (scale tables pass through as void *)
     std::vector<const void *> g;
     std::vector<long long> n;
     std::vector<float *> counts;
@@ -48,23 +311,22 @@ bool usable(const at::Tensor &t, const char *what)
     return true;
 }
 
-// adamw_step(params, state, keys, bits, fp32 entry point, bf16 entry point, lr, beta1, beta2, eps, weight_decay, stream_of)
+// adamw_step(params, state, keys, bits, lr, beta1, beta2, eps, weight_decay)
 //   params: list of Parameters; state: the optimiser's {Parameter: {key: tensor}}; keys: moments in the order of the
-//   library's tables; stream_of(device index) -> raw stream.
+//   library's tables.
 // Returns the parameters that have a gradient and no state; where there are any, nothing has been launched.
-// Otherwise an empty list, or the library's nonzero status.
+// Otherwise an empty list.
 PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 {
     HANDLE_TH_ERRORS
-    if (nargs != 12 || !PyList_Check(args[0]) || !PyDict_Check(args[1]) || !PyTuple_Check(args[2])) {
+    if (nargs != 9 || !PyList_Check(args[0]) || !PyDict_Check(args[1]) || !PyTuple_Check(args[2])) {
         PyErr_SetString(PyExc_TypeError, "adamw_step: (list, dict, tuple, ...)");
         return nullptr;
     }
     PyObject *params = args[0], *state = args[1], *keys = args[2];
     const long bits = PyLong_AsLong(args[3]);
-    void *fn32 = PyLong_AsVoidPtr(args[4]), *fn16 = PyLong_AsVoidPtr(args[5]);
     double hp[5];
-    for (int i = 0; i < 5; ++i) hp[i] = PyFloat_AsDouble(args[6 + i]);
+    for (int i = 0; i < 5; ++i) hp[i] = PyFloat_AsDouble(args[4 + i]);
     if (PyErr_Occurred()) return nullptr;
     const Py_ssize_t nkeys = PyTuple_GET_SIZE(keys);
     if (nkeys != (bits == 8 ? 4 : 2)) {
@@ -162,19 +424,15 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     }
     if (PyList_GET_SIZE(missing.get())) return missing.release();
     for (const Batch &b : batches) {
-        c10::DeviceGuard guard(b.device);
-        THPObjectPtr stream(PyObject_CallFunction(args[11], "i", (int)b.device.index()));
-        if (!stream) return nullptr;
-        void *st = PyLong_AsVoidPtr(stream);
-        if (PyErr_Occurred()) return nullptr;
-        void *fn = b.type == at::kBFloat16 ? fn16 : fn32;
-        const int count = (int)b.p.size();
-        const int rc = bits == 8
-            ? ((adamw8_fn)fn)(count, b.p.data(), b.g.data(), b.s[0].data(), b.s[1].data(), b.s[2].data(), b.s[3].data(),
-                              b.n.data(), hp[0], hp[1], hp[2], hp[3], hp[4], b.step + 1, st)
-            : ((adamw32_fn)fn)(count, b.p.data(), b.g.data(), b.s[0].data(), b.s[1].data(), b.n.data(), hp[0], hp[1], hp[2],
-                               hp[3], hp[4], b.step + 1, st);
-        if (rc) return PyLong_FromLong(rc);
+        const c10::DeviceGuard guard(b.device);
+        const int which = b.type == at::kBFloat16, count = (int)b.p.size();
+        check(bits == 8
+                  ? lib.adamw8[which](count, b.p.data(), b.g.data(), b.s[0].data(), (float *const *)b.s[1].data(), b.s[2].data(),
+                                      (float *const *)b.s[3].data(), b.n.data(), hp[0], hp[1], hp[2], hp[3], hp[4], b.step + 1,
+                                      stream(b.device))
+                  : lib.adamw[which](count, b.p.data(), b.g.data(), (float *const *)b.s[0].data(),
+                                     (float *const *)b.s[1].data(), b.n.data(), hp[0], hp[1], hp[2], hp[3], hp[4], b.step + 1,
+                                     stream(b.device)));
         for (float *f : b.counts) *f = (float)(b.step + 1);
         // the parameters have changed behind torch's back: copies kept of them go by the version
         for (c10::TensorImpl *t : b.changed) t->bump_version();
@@ -183,7 +441,36 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     END_HANDLE_TH_ERRORS
 }
 
-PyMethodDef methods[] = {{"adamw_step", (PyCFunction)(void (*)(void))adamw_step, METH_FASTCALL, nullptr},
+// bind(name -> address): see Library
+PyObject *bind(PyObject *, PyObject *of)
+{
+    HANDLE_TH_ERRORS
+    auto take = [&](auto &fn, const std::string &name) {
+        THPObjectPtr address(PyObject_CallFunction(of, "s", name.c_str()));
+        if (!address) throw python_error();
+        fn = (std::remove_reference_t<decltype(fn)>)PyLong_AsVoidPtr(address);
+    };
+    take(lib.last_error, "erf_last_error");
+    take(lib.norm_ws, "erf_layer_norm_workspace_bytes");
+    take(lib.logp_ws, "erf_log_probs_workspace_bytes");
+    for (int bf16 = 0; bf16 < 2; ++bf16) {
+        const std::string tail = bf16 ? "_bf16" : "";
+        take(lib.norm_fwd[bf16], "erf_layer_norm_forward" + tail);
+        take(lib.norm_bwd[bf16], "erf_layer_norm_backward" + tail);
+        take(lib.logp_fwd[bf16], "erf_log_probs_forward" + tail);
+        take(lib.logp_bwd[bf16], "erf_log_probs_backward" + tail);
+        take(lib.adamw[bf16], "erf_adamw_step" + tail);
+        take(lib.adamw8[bf16], "erf_adamw8_step" + tail);
+    }
+    if (PyErr_Occurred()) throw python_error();
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr},
+                         {"layer_norm", (PyCFunction)(void (*)(void))layer_norm, METH_FASTCALL, nullptr},
+                         {"log_probs", (PyCFunction)(void (*)(void))log_probs, METH_FASTCALL, nullptr},
+                         {"adamw_step", (PyCFunction)(void (*)(void))adamw_step, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

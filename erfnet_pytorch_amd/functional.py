@@ -1274,89 +1274,7 @@ def mse_mean(a, b):
 
 
 # ------------------------------------------------------------------------------ layer norm, log probabilities
-# These calls are often shorter than the host's part in them, so they keep that small: pointers go to the library as
-# plain integers, the device is switched only when another one is current, nothing but allocations and the call itself.
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _call(fn, dev, *args):
-    """fn(*args, current stream of dev) with dev current; raises what the library reports."""
-    if torch._C._cuda_getDevice() == dev.index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    if rc:
-        _lib.check(rc)
-
-
-def _first_order(impl):
-    """backward() of an operator whose gradient has no gradient: torch's once_differentiable refuses a second pass, and is
-    only in the way while no graph of the backward pass is being recorded."""
-    guarded = torch.autograd.function.once_differentiable(impl)
-
-    def backward(ctx, *grads):
-        return (guarded if torch.is_grad_enabled() else impl)(ctx, *grads)
-    return staticmethod(backward)
-
-
-def _norm_forward(x, w, b, eps, image, keep):
-    # rows of C contiguous channels: the last axis as it is, axis 1 of an image as NHWC memory
-    if image:
-        x = _nhwc(x)
-        c = x.shape[1]
-        y = _empty_nhwc(*x.shape, x)
-    else:
-        x = x.contiguous()
-        c = x.shape[-1]
-        y = torch.empty_like(x)
-    rows = x.numel() // c
-    stat = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
-    w, b = _param(w), _param(b)
-    _call(_fn("erf_layer_norm_forward", x), x.device, x.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), _ptr(stat),
-          stat.data_ptr() + 4 * rows if keep else None, rows, c, eps)
-    return x, y, stat
-
-
-def _norm_backward(ctx, gy):
-    x, w, stat = ctx.saved_tensors
-    rows, dev = stat.shape[1], x.device
-    dx = None
-    if ctx.image:
-        c = x.shape[1]
-        gy = _nhwc(gy, x.dtype)
-        if ctx.needs_input_grad[0]:
-            dx = _empty_nhwc(*x.shape, x)
-    else:
-        c = x.shape[-1]
-        gy = gy.to(x.dtype).contiguous()
-        if ctx.needs_input_grad[0]:
-            dx = torch.empty_like(x)
-    tg = _grad_targets(ctx.params, [(c,) if need else None for need in ctx.needs_input_grad[1:3]], dev)
-    dw, db = tg[0][0], tg[1][0]
-    ws, n_ws = None, 0
-    if dw is not None or db is not None:
-        n_ws = _lib.lib().erf_layer_norm_workspace_bytes(rows, c)
-        ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
-    w = _param(w)
-    _call(_fn("erf_layer_norm_backward", x), dev, x.data_ptr(), _ptr(w), stat.data_ptr(), stat.data_ptr() + 4 * rows,
-          gy.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), rows, c, _ptr(ws), n_ws)
-    dw, db = _match_params(_deliver(tg), ctx.params)
-    return dx, dw, db, None, None
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, b, eps, image):
-        x, y, stat = _norm_forward(x, w, b, eps, image, True)
-        ctx.save_for_backward(x, w, stat)
-        ctx.image, ctx.params = image, (w, b)
-        return y
-
-    backward = _first_order(_norm_backward)
-
-
+# The autograd nodes of these two are C++ (csrc/host_ext.cpp): they are often shorter than their host side.
 def _need_gpu(what, x, *others):
     if not x.is_cuda:
         raise RuntimeError(f"{what}: the tensor lives on {x.device}; the kernels run on the GPU only")
@@ -1385,11 +1303,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, dim=-1):
     if not eps >= 0:
         raise ValueError(f"layer_norm: eps must not be negative (got {eps})")
     _need_gpu("layer_norm", x, weight, bias)
-    image = axis != nd - 1
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, float(eps), image)
-    return _norm_forward(x, weight, bias, float(eps), image, False)[1]
+    return _lib.host().layer_norm(x, weight, bias, float(eps), axis != nd - 1)
 
 
 # ------------------------------------------------------------------------------ token log probabilities
@@ -1399,69 +1313,6 @@ class LogProbs(NamedTuple):
     entropy: torch.Tensor
     top_log_probs: torch.Tensor
     top_indices: torch.Tensor
-
-
-def _logp_forward(logits, target, top_k, ignore_index, axis):
-    """The results in the caller's shapes, and what backward needs: the logits as the kernels read them
-    ([outer, V, inner]), the kept statistics and the problem's size."""
-    shape = tuple(logits.shape)
-    nd, v = len(shape), shape[axis]
-    lead, tail = shape[:axis], shape[axis + 1:]
-    inner = 1
-    for n in tail:
-        inner *= n
-    pixels = target.numel()
-    target = target.contiguous()
-    # The pixel kernel gives a thread a pixel; it needs enough of them to fill the card, and keeps up to 8
-    # alternatives in registers.
-    plane = inner > 1 and v <= 256 and top_k <= 8 and pixels >= 4096
-    if plane:
-        x = logits.contiguous()
-        outer, ld, full = pixels // inner, 0, lead + (top_k,) + tail
-    else:
-        x = (logits if axis == nd - 1 else logits.movedim(axis, -1)).reshape(pixels, v)
-        outer, inner, full = pixels, 1, lead + tail + (top_k,)
-        if x.stride(1) != 1 or (outer > 1 and x.stride(0) < v):
-            x = x.contiguous()
-        ld = x.stride(0) if outer > 1 else v
-    dev = x.device
-    lp = torch.empty(target.shape, dtype=torch.float32, device=dev)
-    ent = torch.empty(target.shape, dtype=torch.float32, device=dev)
-    stats = torch.empty(2 * pixels, dtype=torch.float32, device=dev)
-    top = torch.empty(full, dtype=torch.float32, device=dev)
-    idx = torch.empty(full, dtype=torch.int64, device=dev)
-    n_ws = _lib.lib().erf_log_probs_workspace_bytes(outer, v, inner, top_k)
-    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev) if n_ws else None
-    _call(_fn("erf_log_probs_forward", x), dev, x.data_ptr(), target.data_ptr(), lp.data_ptr(), ent.data_ptr(),
-          stats.data_ptr(), top.data_ptr(), idx.data_ptr(), outer, v, inner, ld, top_k, ignore_index, _ptr(ws), n_ws)
-    moved = not plane and axis != nd - 1
-    out = (lp, ent, top.movedim(-1, axis), idx.movedim(-1, axis)) if moved else (lp, ent, top, idx)
-    return out, (x, target, stats, ent, idx), (outer, v, inner, ld, top_k, ignore_index), moved
-
-
-def _logp_backward(ctx, g_lp, g_ent, g_top, _):
-    x, target, stats, ent, idx = ctx.saved_tensors
-    if g_top is not None and ctx.moved:
-        g_top = g_top.movedim(ctx.axis, -1)
-    g_lp, g_ent, g_top = (None if g is None else g.to(torch.float32).contiguous() for g in (g_lp, g_ent, g_top))
-    dx = torch.empty(ctx.moved or ctx.shape, dtype=x.dtype, device=x.device)
-    _call(_fn("erf_log_probs_backward", x), x.device, x.data_ptr(), target.data_ptr(), ent.data_ptr(), stats.data_ptr(),
-          idx.data_ptr(), _ptr(g_lp), _ptr(g_ent), _ptr(g_top), dx.data_ptr(), *ctx.cfg)
-    return (dx.movedim(-1, ctx.axis) if ctx.moved else dx), None, None, None, None
-
-
-class _LogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, target, top_k, ignore_index, axis):
-        out, kept, ctx.cfg, moved = _logp_forward(logits, target, top_k, ignore_index, axis)
-        shape = tuple(logits.shape)
-        ctx.axis, ctx.shape, ctx.moved = axis, shape, moved and shape[:axis] + shape[axis + 1:] + (shape[axis],)
-        ctx.mark_non_differentiable(out[3])
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*kept)
-        return out
-
-    backward = _first_order(_logp_backward)
 
 
 def log_probs(logits, target, top_k=0, dim=-1, ignore_index=-1):
@@ -1493,6 +1344,4 @@ def log_probs(logits, target, top_k=0, dim=-1, ignore_index=-1):
         raise ValueError(f"log_probs: top_k must be in 0..{min(64, v)} (got {top_k})")
     _need_gpu("log_probs", logits, target)
     _materialize_logits(logits)
-    if logits.requires_grad and torch.is_grad_enabled():
-        return LogProbs(*_LogProbs.apply(logits, target, int(top_k), int(ignore_index), axis))
-    return LogProbs(*_logp_forward(logits, target, int(top_k), int(ignore_index), axis)[0])
+    return LogProbs(*_lib.host().log_probs(logits, target, int(top_k), int(ignore_index), axis))

@@ -169,8 +169,6 @@ class AdamW(torch.optim.Optimizer):
 
     ``step`` cannot be captured into a HIP graph (the library refuses): the bias corrections go into the launch."""
 
-    _entry_points = None
-
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
         if lr < 0.0 or eps < 0.0 or weight_decay < 0.0:
             raise ValueError("AdamW: lr, eps and weight_decay must not be negative")
@@ -223,24 +221,17 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        host, fns = _lib.host(), self._entry_points
-        if fns is None:
-            lib, name = _lib.lib(), "erf_adamw_step" if self.state_bits == 32 else "erf_adamw8_step"
-            fns = self._entry_points = tuple(C.cast(getattr(lib, name + s), C.c_void_p).value for s in ("", "_bf16"))
+        host = _lib.host()
         for group in self.param_groups:
             if group.get("amsgrad") or group.get("maximize") or not group.get("decoupled_weight_decay", True):
                 raise NotImplementedError("erfnet_pytorch_amd.optim.AdamW: amsgrad / maximize / L2 weight decay are "
                                           "not implemented (Adam has the latter)")
             b1, b2 = group["betas"]
-            args = (group["params"], self.state, self._moments, self.state_bits, *fns, float(group["lr"]), float(b1),
-                    float(b2), float(group["eps"]), float(group["weight_decay"]), torch._C._cuda_getCurrentRawStream)
-            left = host.adamw_step(*args)
-            if left:                    # parameters that have their first gradient
-                if isinstance(left, int):
-                    _lib.check(left)
-                for p in left:
+            args = (group["params"], self.state, self._moments, self.state_bits, float(group["lr"]), float(b1), float(b2),
+                    float(group["eps"]), float(group["weight_decay"]))
+            first = host.adamw_step(*args)
+            if first:                   # parameters that have their first gradient: nothing has been launched yet
+                for p in first:
                     self.state[p].update(self._new_state(p))
-                left = host.adamw_step(*args)
-                if left:
-                    _lib.check(left)
+                host.adamw_step(*args)
         return loss

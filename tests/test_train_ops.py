@@ -424,6 +424,19 @@ def test_log_probs_agree_with_cross_entropy():
     assert (a.grad - b.grad).abs().max() <= 2 * 256 * 37 * U / n
 
 
+@gpu
+@pytest.mark.parametrize("op", ["layer_norm", "log_probs"])
+def test_gradients_are_not_differentiable(op):
+    from erfnet_pytorch_amd import functional as hipf
+    x = torch.randn(4, 32, generator=torch.Generator().manual_seed(1)).to(DEV).requires_grad_()
+    y = hipf.layer_norm(x) if op == "layer_norm" else hipf.log_probs(x, torch.zeros(4, dtype=torch.int64, device=DEV)).log_prob
+    plain, = torch.autograd.grad((y * y).sum(), x, retain_graph=True)
+    dx, = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+    assert torch.equal(dx, plain)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(dx.sum(), x)
+
+
 # ================================================================================ AdamW
 HP = dict(lr=3e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
 
