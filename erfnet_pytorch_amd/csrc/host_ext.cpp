@@ -150,9 +150,10 @@ variable_list logp_forward(const Tensor &logits, const Tensor &target0, LogpShap
     const int64_t pixels = target.numel();
     const c10::DeviceGuard guard(logits.device());
     std::vector<int64_t> full;
-    // The pixel kernel gives a thread a pixel; it needs enough of them to fill the card, and keeps up to 8
-    // alternatives in registers.
-    const bool plane = s.inner > 1 && s.v <= 256 && s.top_k <= ERF_LOG_PROBS_MAX_TOP_PIXELS && pixels >= 4096;
+    // The pixel kernel gives a thread a pixel: its time goes with the class count until the pixels fill the card.  Bringing
+    // the classes together first and giving a wave a row goes with the pixels (fp32, top 2, 150 classes: 20 and 13 us at
+    // 4096 pixels, 20 and 36 at 16384; 20 classes: 4.5 and 8.5 at 1024, 4.8 and 24 at 16384).
+    const bool plane = s.inner > 1 && s.top_k <= ERF_LOG_PROBS_MAX_TOP_PIXELS && (s.v <= 32 || pixels >= 64 * s.v);
     s.moved = !plane && s.axis != nd - 1;
     if (plane) {
         x = logits.contiguous();

@@ -29,7 +29,7 @@ struct LpDesc {
     long long *top_idx;
     long long rows;             // row kernels: rows; pixel kernels: outer * inner
     long long ld;               // row kernels: elements from row to row
-    long long inner;            // pixel kernels
+    long long inner, group, next;   // pixel kernels: pixel p is element (p / inner) * group + p % inner, its classes `next` apart
     long long ignore;
     int V, k;
     int splits, seg;            // row kernels: blocks per row and elements of each
@@ -474,16 +474,70 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_rows_bwd_kernel(const LpDesc d)
     }
 }
 
+// Many short rows: a block takes LP_SHORT_ROWS of them as one run of elements, so that all lanes work whatever V is, with
+// what a row's entries need of it in shared memory.
+#define LP_SHORT_ROWS 64
+template <typename T>
+__global__ __launch_bounds__(LP_BLOCK) void lp_short_rows_bwd_kernel(const LpDesc d)
+{
+    __shared__ float m[LP_SHORT_ROWS], log_s[LP_SHORT_ROWS], G[LP_SHORT_ROWS], gh[LP_SHORT_ROWS], H[LP_SHORT_ROWS], glp[LP_SHORT_ROWS];
+    __shared__ int target[LP_SHORT_ROWS];
+    const long long row0 = (long long)blockIdx.x * LP_SHORT_ROWS;
+    const int rows = d.rows - row0 < LP_SHORT_ROWS ? (int)(d.rows - row0) : LP_SHORT_ROWS, V = d.V, k = d.g_top ? d.k : 0;
+    // four threads add up a row's upstream gradients
+    const int mine = threadIdx.x >> 2, part = threadIdx.x & 3;
+    {
+        float g = 0.0f;
+        if (mine < rows)
+            for (int j = part; j < k; j += 4) g += d.g_top[(row0 + mine) * d.k + j];
+        g = wave_sum(g, 4);
+        if (mine < rows && part == 0) {
+            const long long row = row0 + mine;
+            const float2 st = d.stats[row];
+            long long t = d.target[row];
+            if (t == d.ignore || t < 0 || t >= V) t = -1;
+            const float a = t >= 0 && d.g_lp ? d.g_lp[row] : 0.0f;
+            m[mine] = st.x;
+            log_s[mine] = st.y;
+            G[mine] = g + a;
+            gh[mine] = d.g_h ? d.g_h[row] : 0.0f;
+            H[mine] = d.entropy[row];
+            glp[mine] = a;
+            target[mine] = (int)t;
+        }
+    }
+    __syncthreads();
+    const T *x = (const T *)d.x + row0 * d.ld;
+    T *dx = (T *)d.dx + row0 * V;
+    for (int e = threadIdx.x; e < rows * V; e += LP_BLOCK) {
+        const int r = e / V, c = e - r * V;
+        const float g = lp_grad(Vec16<T>::get(x + r * d.ld + c), m[r], log_s[r], G[r], gh[r], H[r]);
+        Vec16<T>::put(dx + e, log_s[r] == -INFINITY ? 0.0f : c == target[r] ? g + glp[r] : g);
+    }
+    if (!k) return;
+    // the alternatives' entries again, with what was gathered there (the target's among them has both)
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * k; e += LP_BLOCK) {
+        const int r = e / k, j = e - r * k;
+        if (log_s[r] == -INFINITY) continue;
+        const long long at = (row0 + r) * d.k + j;
+        const int c = (int)d.top_idx[at];
+        const float g = lp_grad(Vec16<T>::get(x + r * d.ld + c), m[r], log_s[r], G[r], gh[r], H[r]) + d.g_top[at];
+        Vec16<T>::put(dx + (long long)r * V + c, c == target[r] ? g + glp[r] : g);
+    }
+}
+
 // ---------------------------------------------------------------------------------- pixels: [outer][V][inner]
 // A thread takes one pixel and walks the classes; neighbouring threads take neighbouring pixels.  K >= k alternatives
-// in registers.
+// in registers.  Forward, short rows (inner = 1) are pixels too: a wave's loads then lie a row apart, but its 64 rows of a
+// few classes stay in the first-level cache from one class to the next.
 template <typename T, int K>
 __global__ __launch_bounds__(LP_BLOCK) void lp_pixels_kernel(const LpDesc d)
 {
     const long long p = (long long)blockIdx.x * LP_BLOCK + threadIdx.x;
     if (p >= d.rows) return;
     const long long n = p / d.inner, q = p - n * d.inner;
-    const T *x = (const T *)d.x + n * d.V * d.inner + q;
+    const T *x = (const T *)d.x + n * d.group + q;
     LpSums r = {LP_LOWEST, 0.0f, 0.0f};
     unsigned key[K > 0 ? K : 1];
     int idx[K > 0 ? K : 1];
@@ -494,7 +548,7 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_pixels_kernel(const LpDesc d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int cc = c + i < d.V ? c + i : d.V - 1;
-            v[i] = Vec16<T>::get(x + (long long)cc * d.inner);
+            v[i] = Vec16<T>::get(x + cc * d.next);
         }
         float m = r.m;
 #pragma unroll
@@ -531,7 +585,7 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_pixels_kernel(const LpDesc d)
     d.entropy[p] = none ? 0.0f : log_s - r.a / r.s;
     const long long t = d.target[p];
     float lp = 0.0f;
-    if (t != d.ignore && t >= 0 && t < d.V) lp = none ? -INFINITY : Vec16<T>::get(x + t * d.inner) - r.m - log_s;
+    if (t != d.ignore && t >= 0 && t < d.V) lp = none ? -INFINITY : Vec16<T>::get(x + t * d.next) - r.m - log_s;
     d.log_prob[p] = lp;
     if (K > 0) {
 #pragma unroll
@@ -550,8 +604,8 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_pixels_bwd_kernel(const LpDesc d)
     const long long p = (long long)blockIdx.x * LP_BLOCK + threadIdx.x;
     if (p >= d.rows) return;
     const long long n = p / d.inner, q = p - n * d.inner;
-    const T *x = (const T *)d.x + n * d.V * d.inner + q;
-    T *dx = (T *)d.dx + n * d.V * d.inner + q;
+    const T *x = (const T *)d.x + n * d.group + q;
+    T *dx = (T *)d.dx + n * d.V * d.inner + q;      // (dense, whatever the stride between rows of x)
     const float2 st = d.stats[p];
     const float H = d.entropy[p], gh = d.g_h ? d.g_h[p] : 0.0f;
     const bool none = st.y == -INFINITY;
@@ -570,7 +624,7 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_pixels_bwd_kernel(const LpDesc d)
     }
 #pragma unroll 4
     for (int c = 0; c < d.V; ++c) {
-        float g = lp_grad(Vec16<T>::get(x + (long long)c * d.inner), st.x, st.y, G, gh, H);
+        float g = lp_grad(Vec16<T>::get(x + c * d.next), st.x, st.y, G, gh, H);
         if (c == (int)t) g += glp;
 #pragma unroll
         for (int j = 0; j < K; ++j) g += idx[j] == c ? gt[j] : 0.0f;

@@ -132,8 +132,26 @@ int norm_backward(const void *x, const float *w, const float *mean, const float 
 
 // ================================================================================ token log probabilities
 #define LP_MAX_CLASSES (1 << 30)
+// Rows of up to LP_SHORT classes leave most of a wave idle, and where there are many of them that counts: forward from 64 rows
+// a class on (us, a thread a row / a wave a row, fp32, top 2: 262144 x 20 10 / 249, 262144 x 100 75 / 247, 16384 x 100 16 / 20,
+// 1024 x 100 15 / 5), backward from 256 (as one run of elements / a wave a row: 262144 x 20 13 / 81, 262144 x 100 42 / 85,
+// 16384 x 64 7.4 / 6.7, 16384 x 200 20 / 8).
+#define LP_SHORT 128
+#define LP_SHORT_FORWARD 64ll
+#define LP_SHORT_BACKWARD 256ll
 
-// Blocks per row: a wave takes a row of up to 2048 classes; longer ones take whole blocks of at least 4096 classes, several to
+// Forward: a thread takes a whole pixel, and a short row of many.
+bool lp_by_thread(long long outer, int V, long long inner, int k)
+{
+    return inner > 1 || (V <= LP_SHORT && k <= ERF_LOG_PROBS_MAX_TOP_PIXELS && outer >= LP_SHORT_FORWARD * V);
+}
+// Forward: a wave takes a row of up to 4096 classes (8192 x 4000 bf16, top 8: 23 us, 42 with a block a row; 8192 x 8000 fp32: 65
+// and 55); backward, which has no results to join, of up to 1024 (8192 x 1000 bf16: 8.0 and 11.6 us, 8192 x 4000: 23.1 and 21.8).
+#define LP_WAVE_FORWARD 4096
+#define LP_WAVE_BACKWARD 1024
+#define LP_BACKWARD_SEGMENT 8192
+
+// Forward, blocks per row: longer rows take whole blocks of at least 4096 classes, several to
 // a row until they fill the card twice (2048 are resident), or once where every block also finds alternatives
 // (2047 x 100003 bf16: 82 us with two rounds, 95 with one; with 8 alternatives 116 and 114, and 123 with four rounds).
 struct LpPlan {
@@ -142,7 +160,7 @@ struct LpPlan {
 };
 LpPlan lp_plan(long long rows, int V, int k)
 {
-    LpPlan p = {V <= 2048, 1, V};
+    LpPlan p = {V <= LP_WAVE_FORWARD, 1, V};
     if (p.wave) return p;
     const long long want = ((k ? 2048 : 4096) + rows - 1) / std::max<long long>(rows, 1);
     p.splits = (int)std::min<long long>(std::max<long long>(want, 1), (V + 4095) / 4096);
@@ -152,7 +170,7 @@ LpPlan lp_plan(long long rows, int V, int k)
 }
 size_t lp_ws(long long outer, int V, long long inner, int k)
 {
-    if (inner > 1) return 0;
+    if (lp_by_thread(outer, V, inner, k)) return 0;
     const LpPlan p = lp_plan(outer, V, k);
     return p.splits > 1 ? (size_t)outer * p.splits * (sizeof(float4) + (size_t)k * 8) : 0;
 }
@@ -166,7 +184,7 @@ int lp_check(const char *what, long long outer, int V, long long inner, int k)
     // one block per 256 pixels or per (row, segment): the grid must fit 31 bits
     if (outer > (1ll << 40) / inner) return fail("%s: too many rows", what);
     const long long blocks = inner > 1 ? (outer * inner + LP_BLOCK - 1) / LP_BLOCK
-                                       : V <= 2048 ? (outer + 3) / 4 : outer * ((V + 8191) / 8192);
+                                       : outer * ((V + LP_BACKWARD_SEGMENT - 1) / LP_BACKWARD_SEGMENT);
     if (blocks >= (1ll << 31)) return fail("%s: too many rows", what);
     return 0;
 }
@@ -185,7 +203,9 @@ int lp_forward(const void *x, const long long *target, float *log_prob, float *e
     d.x = x; d.target = target; d.log_prob = log_prob; d.entropy = entropy; d.stats = (float2 *)stats;
     d.top_lp = top_lp; d.top_idx = top_idx; d.rows = outer * inner; d.ld = ld; d.inner = inner; d.ignore = ignore;
     d.V = V; d.k = k;
-    if (inner > 1) {
+    if (lp_by_thread(outer, V, inner, k)) {
+        d.group = inner > 1 ? V * inner : ld;
+        d.next = inner;
         const unsigned blocks = (unsigned)((d.rows + LP_BLOCK - 1) / LP_BLOCK);
         if (k == 0) lp_pixels_kernel<T, 0><<<blocks, LP_BLOCK, 0, st>>>(d);
         else if (k == 1) lp_pixels_kernel<T, 1><<<blocks, LP_BLOCK, 0, st>>>(d);
@@ -234,6 +254,8 @@ int lp_backward(const void *x, const long long *target, const float *entropy, co
     d.top_idx = const_cast<long long *>(top_idx); d.g_lp = g_lp; d.g_h = g_h; d.g_top = g_top; d.dx = dx;
     d.rows = outer * inner; d.ld = ld; d.inner = inner; d.ignore = ignore; d.V = V; d.k = k;
     if (inner > 1) {
+        d.group = V * inner;
+        d.next = inner;
         const unsigned blocks = (unsigned)((d.rows + LP_BLOCK - 1) / LP_BLOCK);
         if (!g_top || k == 0) lp_pixels_bwd_kernel<T, 0><<<blocks, LP_BLOCK, 0, st>>>(d);
         else if (k <= 2) lp_pixels_bwd_kernel<T, 2><<<blocks, LP_BLOCK, 0, st>>>(d);
@@ -241,10 +263,12 @@ int lp_backward(const void *x, const long long *target, const float *entropy, co
         LAUNCHED("lp_pixels_bwd_kernel");
         return 0;
     }
-    if (V <= 2048) {
+    if (V <= LP_SHORT && outer >= LP_SHORT_BACKWARD * V) {
+        lp_short_rows_bwd_kernel<T><<<(unsigned)((outer + LP_SHORT_ROWS - 1) / LP_SHORT_ROWS), LP_BLOCK, 0, st>>>(d);
+    } else if (V <= LP_WAVE_BACKWARD) {
         lp_rows_bwd_kernel<T, 64><<<(unsigned)((outer + 3) / 4), LP_BLOCK, 0, st>>>(d);
     } else {
-        d.seg = 8192;
+        d.seg = LP_BACKWARD_SEGMENT;
         d.splits = (V + d.seg - 1) / d.seg;
         lp_rows_bwd_kernel<T, 256><<<(unsigned)(outer * d.splits), LP_BLOCK, 0, st>>>(d);
     }

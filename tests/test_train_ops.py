@@ -268,7 +268,8 @@ def lp_case(n, v, kind, k, seed=0, masked=True, ties=False):
 
 
 LP_ROWS = [(1, 1, 1), (1, 2, 2), (5, 3, 0), (4, 7, 7), (9, 64, 64), (6, 65, 5), (256, 1000, 5), (3, 1000, 64), (2, 2048, 20),
-           (2, 2049, 20), (3, 4096, 0), (1, 5000, 64), (3, 50021, 8), (1, 131072, 20), (40, 8193, 3), (1100, 2500, 2)]
+           (2, 2049, 20), (3, 4096, 0), (1, 5000, 64), (3, 50021, 8), (1, 131072, 20), (40, 8193, 3), (1100, 2500, 2), (5121, 20, 3), (1281, 5, 0), (4099, 64, 8), (6401, 100, 9), (8200, 128, 5), (32769, 128, 9),
+           (16390, 64, 33), (8300, 129, 1), (70, 1024, 4), (70, 1025, 4), (40, 4096, 9), (40, 4097, 9)]
 
 
 @gpu
