@@ -19,8 +19,8 @@ struct NormDesc {
     const float *w, *b;         // [C] or null
     float *mean, *rstd;         // [rows]; forward may leave them null
     float *partial;             // backward: [blocks][2][C] sums of g xhat and of g
-    long long rows;
-    int C, lanes, lane_bits;    // lanes (a power of two) share a row in the wave kernels
+    long long rows, safe_rows;  // of the first safe_rows rows, a vector that begins in the row ends in the tensor
+    int C;
     float eps;
 };
 
@@ -42,34 +42,58 @@ __device__ __forceinline__ float norm_block_sum(float v, float *red)
     return s;
 }
 
-// The vectors of one row that a thread holds: R of them, `threads` apart, this thread's first at vector `me`.
-template <typename T, int R>
-__device__ __forceinline__ void norm_load(u32x4 (&raw)[R], const void *base, long long row, int C, int me, int threads)
+// The vectors of one row that a thread holds: R of them, `threads` apart, this thread's first at vector `me`.  EVEN: C is a
+// multiple of the vector.  Otherwise a row's last vector reads on into the next rows (where there are any: safe_rows), and
+// what it reads of them is cut off where it is unpacked (norm_unpack): the load itself has no wait.
+template <typename T, int R, bool EVEN>
+__device__ __forceinline__ void norm_load(u32x4 (&raw)[R], const NormDesc &d, const void *base, long long row, int me, int threads)
 {
-    const T *x = (const T *)base + row * C;
+    const T *x = (const T *)base + row * d.C;
+    const bool inside = row < d.safe_rows;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int c = (r * threads + me) * Vec16<T>::N;
-        raw[r] = ld16(x + c, C - c);
+        if constexpr (EVEN) {
+            raw[r] = (u32x4){0u, 0u, 0u, 0u};
+            if (c < d.C) raw[r] = reinterpret_cast<const typename Vec16<T>::Raw *>(x + c)->v;
+        } else {
+            raw[r] = ld16(x + c, d.C - c, inside);
+        }
+    }
+}
+template <typename T, bool EVEN> __device__ __forceinline__ void norm_unpack(u32x4 raw, float (&f)[Vec16<T>::N], int left)
+{
+    if (!EVEN && left < Vec16<T>::N) raw = first16<T>(raw, left);
+    Vec16<T>::unpack(raw, f);
+}
+template <typename T, bool EVEN> __device__ __forceinline__ void norm_store(T *p, const float (&f)[Vec16<T>::N], int left)
+{
+    if constexpr (EVEN) {
+        if (left > 0) reinterpret_cast<typename Vec16<T>::Raw *>(p)->v = Vec16<T>::pack(f);
+    } else {
+        st16(p, f, left);
     }
 }
 
-// GROUP = false: one row per `lanes` lanes of a wave; true: one row per block.  Every thread walks over rows and has
+// LANES > 0: one row per LANES lanes of a wave; 0: one row per block.  Every thread walks over rows and has
 // the next row's loads in flight while it works on one, so the latency of memory and of the two sums behind one
-// another overlaps with the loads; weight and bias stay in registers.
-template <typename T, int R, bool BLOCK>
-__global__ __launch_bounds__(BLOCK ? 1024 : NORM_BLOCK) void norm_fwd_kernel(const NormDesc d)
+// another overlaps with the loads; weight and bias stay in registers.  (Short rows are bound by instructions as much as by
+// memory: with the lane count and the shape of a row's end known to the compiler, 990099 x 101 fp32 takes 173 us instead
+// of 209.)
+template <typename T, int R, int LANES, bool EVEN>
+__global__ __launch_bounds__(LANES ? NORM_BLOCK : 1024) void norm_fwd_kernel(const NormDesc d)
 {
+    constexpr bool BLOCK = LANES == 0;
     constexpr int N = Vec16<T>::N;
     __shared__ float red[2][16];
-    const int C = d.C, threads = BLOCK ? (int)blockDim.x : d.lanes;
-    const int me = BLOCK ? (int)threadIdx.x : (int)threadIdx.x & (d.lanes - 1);
-    const int rows_per_block = BLOCK ? 1 : NORM_BLOCK >> d.lane_bits;
+    const int C = d.C, threads = BLOCK ? (int)blockDim.x : LANES;
+    const int me = BLOCK ? (int)threadIdx.x : (int)threadIdx.x & (LANES - 1);
+    constexpr int rows_per_block = BLOCK ? 1 : NORM_BLOCK / (BLOCK ? 1 : LANES);
     const long long stride = (long long)gridDim.x * rows_per_block;
-    long long row = (long long)blockIdx.x * rows_per_block + (BLOCK ? 0 : threadIdx.x >> d.lane_bits);
+    long long row = (long long)blockIdx.x * rows_per_block + (BLOCK ? 0 : threadIdx.x / (BLOCK ? 1 : LANES));
     if (row >= d.rows) return;                  // (in a block kernel the grid has no more blocks than rows)
     u32x4 next[R];
-    norm_load<T, R>(next, d.x, row, C, me, threads);
+    norm_load<T, R, EVEN>(next, d, d.x, row, me, threads);
     float w[R][N], b[R][N];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -85,12 +109,12 @@ __global__ __launch_bounds__(BLOCK ? 1024 : NORM_BLOCK) void norm_fwd_kernel(con
         float v[R][N], s = 0.0f;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            Vec16<T>::unpack(next[r], v[r]);
+            norm_unpack<T, EVEN>(next[r], v[r], C - (r * threads + me) * N);
 #pragma unroll
             for (int i = 0; i < N; ++i) s += v[r][i];
         }
-        if (row + stride < d.rows) norm_load<T, R>(next, d.x, row + stride, C, me, threads);
-        const float mean = norm_mean(BLOCK ? norm_block_sum(s, red[0]) : wave_sum(s, d.lanes), (float)C, inv_c);
+        if (row + stride < d.rows) norm_load<T, R, EVEN>(next, d, d.x, row + stride, me, threads);
+        const float mean = norm_mean(BLOCK ? norm_block_sum(s, red[0]) : wave_sum(s, LANES), (float)C, inv_c);
         float q = 0.0f;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -101,7 +125,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : NORM_BLOCK) void norm_fwd_kernel(con
                 q += v[r][i] * v[r][i];
             }
         }
-        const float rstd = rsqrtf((BLOCK ? norm_block_sum(q, red[1]) : wave_sum(q, d.lanes)) * inv_c + d.eps);
+        const float rstd = rsqrtf((BLOCK ? norm_block_sum(q, red[1]) : wave_sum(q, LANES)) * inv_c + d.eps);
         if (me == 0 && d.mean) { d.mean[row] = mean; d.rstd[row] = rstd; }
         T *y = (T *)d.y + row * C;
 #pragma unroll
@@ -109,7 +133,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : NORM_BLOCK) void norm_fwd_kernel(con
             const int c = (r * threads + me) * N;
 #pragma unroll
             for (int i = 0; i < N; ++i) v[r][i] = v[r][i] * rstd * w[r][i] + b[r][i];
-            if (c < C) st16(y + c, v[r], C - c);
+            norm_store<T, EVEN>(y + c, v[r], C - c);
         }
     }
 }
@@ -118,23 +142,24 @@ __global__ __launch_bounds__(BLOCK ? 1024 : NORM_BLOCK) void norm_fwd_kernel(con
 // all rows it meets; the block's sums go to partial, and norm_grad_sum_kernel adds the blocks in order.
 // THREADS: most threads of a block kernel (0: wave kernel).  1024 of them have 128 registers each, which hold the sums
 // but neither the weight nor the next row's loads: AHEAD is off there.
-template <typename T, int R, int THREADS>
+template <typename T, int R, int LANES, int THREADS, bool EVEN>
 __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kernel(const NormDesc d)
 {
     constexpr bool BLOCK = THREADS != 0, AHEAD = THREADS != 1024;
+    static_assert(BLOCK == (LANES == 0), "one of the two");
     constexpr int N = Vec16<T>::N;
     extern __shared__ float acc[];              // wave kernel: [4 waves][2][C]
     __shared__ float red[2][2][16];
-    const int C = d.C, threads = BLOCK ? (int)blockDim.x : d.lanes;
-    const int me = BLOCK ? (int)threadIdx.x : (int)threadIdx.x & (d.lanes - 1);
-    const int rows_per_block = BLOCK ? 1 : NORM_BLOCK >> d.lane_bits;
+    const int C = d.C, threads = BLOCK ? (int)blockDim.x : LANES;
+    const int me = BLOCK ? (int)threadIdx.x : (int)threadIdx.x & (LANES - 1);
+    constexpr int rows_per_block = BLOCK ? 1 : NORM_BLOCK / (BLOCK ? 1 : LANES);
     const long long stride = (long long)gridDim.x * rows_per_block;
-    long long row = (long long)blockIdx.x * rows_per_block + (BLOCK ? 0 : threadIdx.x >> d.lane_bits);
+    long long row = (long long)blockIdx.x * rows_per_block + (BLOCK ? 0 : threadIdx.x / (BLOCK ? 1 : LANES));
     u32x4 nx[R], ng[R];
     float nmean = 0.0f, nrstd = 0.0f;
     auto fetch = [&](long long at) __attribute__((always_inline)) {
-        norm_load<T, R>(nx, d.x, at, C, me, threads);
-        norm_load<T, R>(ng, d.gy, at, C, me, threads);
+        norm_load<T, R, EVEN>(nx, d, d.x, at, me, threads);
+        norm_load<T, R, EVEN>(ng, d, d.gy, at, me, threads);
         nmean = d.mean[at];
         nrstd = d.rstd[at];
     };
@@ -159,8 +184,8 @@ __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kerne
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int c = (r * threads + me) * N;
-            Vec16<T>::unpack(nx[r], h[r]);
-            Vec16<T>::unpack(ng[r], g[r]);              // zero beyond the row: nothing below counts it
+            norm_unpack<T, EVEN>(nx[r], h[r], C - c);
+            norm_unpack<T, EVEN>(ng[r], g[r], C - c);         // zero beyond the row: nothing below counts it
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 h[r][i] = (h[r][i] - mean) * rstd;
@@ -172,8 +197,8 @@ __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kerne
             }
         }
         if (AHEAD && row + stride < d.rows) fetch(row + stride);
-        s0 = wave_sum(s0, BLOCK ? 64 : d.lanes);
-        s1 = wave_sum(s1, BLOCK ? 64 : d.lanes);
+        s0 = wave_sum(s0, BLOCK ? 64 : LANES);
+        s1 = wave_sum(s1, BLOCK ? 64 : LANES);
         if (BLOCK) {
             // both sums behind one barrier; the slots alternate, so a wave that is a row ahead cannot overwrite them
             if ((threadIdx.x & 63) == 0) { red[turn][0][threadIdx.x >> 6] = s0; red[turn][1][threadIdx.x >> 6] = s1; }
@@ -189,7 +214,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kerne
             const int c = (r * threads + me) * N;
 #pragma unroll
             for (int i = 0; i < N; ++i) g[r][i] = rstd * (g[r][i] - s0 - h[r][i] * s1);
-            if (c < C && d.y) st16(dx + c, g[r], C - c);
+            if (d.y) norm_store<T, EVEN>(dx + c, g[r], C - c);
         }
     }
     if (!d.partial) return;
@@ -212,7 +237,8 @@ __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kerne
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float a = dw[r][i], b = db[r][i];
-            for (int o = threads; o < 64; o <<= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+#pragma unroll
+            for (int o = BLOCK ? 64 : LANES; o < 64; o <<= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
             if ((threadIdx.x & 63) < threads && c + i < C) { mine[c + i] = a; mine[C + c + i] = b; }
         }
     }

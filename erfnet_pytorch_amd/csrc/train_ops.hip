@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 namespace {
 
@@ -39,13 +40,32 @@ template <typename T> NormPlan norm_plan(int C)
     NormPlan p = {true, 1, 64, NORM_BLOCK};
     if (vecs <= 64 * most) {
         while (p.rounds * 64 < vecs) p.rounds *= 2;
-        p.lanes = 1 << log2_up((vecs + p.rounds - 1) / p.rounds);
+        p.lanes = std::max(2, 1 << log2_up((vecs + p.rounds - 1) / p.rounds));      // (64 where rounds > 1)
         return p;
     }
     p.wave = false;
     p.rounds = most;
     p.threads = ((vecs + most - 1) / most + 63) / 64 * 64;
     return p;
+}
+template <int V> using Int = std::integral_constant<int, V>;
+// launch(even, rounds, lanes) with the plan's values as compile-time constants; lanes = 0: a block per row
+template <typename T, typename F> void norm_by_shape(const NormPlan &p, int C, F launch)
+{
+    auto with = [&](auto even) {
+        constexpr int most = 16 / Vec16<T>::N;
+        if (!p.wave) launch(even, Int<most>(), Int<0>());
+        else if (p.rounds == most && most > 2) launch(even, Int<most>(), Int<64>());
+        else if (p.rounds == 2) launch(even, Int<2>(), Int<64>());
+        else if (p.lanes == 64) launch(even, Int<1>(), Int<64>());
+        else if (p.lanes == 32) launch(even, Int<1>(), Int<32>());
+        else if (p.lanes == 16) launch(even, Int<1>(), Int<16>());
+        else if (p.lanes == 8) launch(even, Int<1>(), Int<8>());
+        else if (p.lanes == 4) launch(even, Int<1>(), Int<4>());
+        else launch(even, Int<1>(), Int<2>());
+    };
+    if (C % Vec16<T>::N == 0) with(std::true_type());
+    else with(std::false_type());
 }
 // Blocks that walk over the rows: as many as the card holds at once, `threads` of them on a compute unit.  Backward takes
 // at least `turns` rows a thread beyond one block per unit, so that the blocks' partial sums stay a small part of its traffic.
@@ -78,13 +98,11 @@ int norm_forward(const void *x, const float *w, const float *b, void *y, float *
     NormDesc d;
     memset(&d, 0, sizeof(d));
     d.x = x; d.y = y; d.w = w; d.b = b; d.mean = mean; d.rstd = rstd;
-    d.rows = rows; d.C = C; d.eps = eps; d.lanes = p.lanes; d.lane_bits = log2_up(p.lanes);
+    d.rows = rows; d.safe_rows = rows - (Vec16<T>::N - 2 + C) / C; d.C = C; d.eps = eps;
     const int blocks = NORM_FWD_BLOCKS(p, rows);
-    constexpr int most = 16 / Vec16<T>::N;
-    if (!p.wave) norm_fwd_kernel<T, most, true><<<blocks, p.threads, 0, st>>>(d);
-    else if (p.rounds == 1) norm_fwd_kernel<T, 1, false><<<blocks, NORM_BLOCK, 0, st>>>(d);
-    else if (p.rounds == 2) norm_fwd_kernel<T, 2, false><<<blocks, NORM_BLOCK, 0, st>>>(d);
-    else norm_fwd_kernel<T, most, false><<<blocks, NORM_BLOCK, 0, st>>>(d);
+    norm_by_shape<T>(p, C, [&](auto even, auto rounds, auto lanes) {
+        norm_fwd_kernel<T, rounds, lanes, even><<<blocks, p.threads, 0, st>>>(d);
+    });
     LAUNCHED("norm_fwd_kernel");
     return 0;
 }
@@ -105,22 +123,21 @@ int norm_backward(const void *x, const float *w, const float *mean, const float 
     if (!dx && !params) return 0;
     const NormPlan p = norm_plan<T>(C);
     const int blocks = NORM_BWD_BLOCKS(p, rows);
-    constexpr int most = 16 / Vec16<T>::N;
     NormDesc d;
     memset(&d, 0, sizeof(d));
     d.x = x; d.gy = gy; d.y = dx; d.w = w; d.mean = const_cast<float *>(mean); d.rstd = const_cast<float *>(rstd);
-    d.rows = rows; d.C = C; d.lanes = p.lanes; d.lane_bits = log2_up(p.lanes);
+    d.rows = rows; d.safe_rows = rows - (Vec16<T>::N - 2 + C) / C; d.C = C;
     if (params) {
         if (blocks && (!ws || ws_bytes < norm_ws<T>(rows, C))) return fail("layer norm backward: workspace too small");
         d.partial = (float *)ws;
     }
     if (blocks) {
         const size_t lds = params && p.wave ? (size_t)8 * C * sizeof(float) : 0;
-        if (!p.wave && p.threads > 512) norm_bwd_kernel<T, most, 1024><<<blocks, p.threads, 0, st>>>(d);
-        else if (!p.wave) norm_bwd_kernel<T, most, 512><<<blocks, p.threads, 0, st>>>(d);
-        else if (p.rounds == 1) norm_bwd_kernel<T, 1, 0><<<blocks, NORM_BLOCK, lds, st>>>(d);
-        else if (p.rounds == 2) norm_bwd_kernel<T, 2, 0><<<blocks, NORM_BLOCK, lds, st>>>(d);
-        else norm_bwd_kernel<T, most, 0><<<blocks, NORM_BLOCK, lds, st>>>(d);
+        norm_by_shape<T>(p, C, [&](auto even, auto rounds, auto lanes) {
+            if constexpr (lanes > 0) norm_bwd_kernel<T, rounds, lanes, 0, even><<<blocks, NORM_BLOCK, lds, st>>>(d);
+            else if (p.threads > 512) norm_bwd_kernel<T, rounds, 0, 1024, even><<<blocks, p.threads, 0, st>>>(d);
+            else norm_bwd_kernel<T, rounds, 0, 512, even><<<blocks, p.threads, 0, st>>>(d);
+        });
         LAUNCHED("norm_bwd_kernel");
     }
     if (params) {
