@@ -165,7 +165,9 @@ class AdamW(torch.optim.Optimizer):
     ``state_bits=8``: both moments as float8 (e4m3) with one fp32 scale per 256 consecutive elements — ``exp_avg``,
     ``exp_avg_scale`` and, as the square root of the second moment, ``exp_avg_sq_root``, ``exp_avg_sq_root_scale`` (value =
     code * scale): 2 bytes an element held instead of 8.  The update itself uses the moments before they are
-    rounded.  ``load_state_dict`` takes the state of an optimiser with the same ``state_bits`` only.
+    rounded.  ``load_state_dict`` takes the state of an optimiser with the same ``state_bits`` only.  On a flat buffer
+    that holds several parameters (``ddp.GradientReducer.flatten_parameters``) the 256 elements of a scale run across them:
+    fp32 moments give the update of the separate tensors bit for bit, 8-bit ones to their rounding.
 
     ``step`` cannot be captured into a HIP graph (the library refuses): the bias corrections go into the launch."""
 
@@ -180,6 +182,13 @@ class AdamW(torch.optim.Optimizer):
                                       maximize=False, foreach=None, capturable=False, differentiable=False,
                                       fused=None, decoupled_weight_decay=True))
         self.defaults["state_bits"] = state_bits        # (what a copied or unpickled optimiser keeps)
+
+    def add_param_group(self, param_group):
+        params = param_group["params"]
+        params = [params] if isinstance(params, torch.Tensor) else list(params)
+        if len({id(p[1] if isinstance(p, tuple) else p) for p in params}) != len(params):
+            raise ValueError("AdamW: a parameter appears twice in one group; its two updates would race")
+        super().add_param_group({**param_group, "params": params})
 
     @property
     def state_bits(self):

@@ -203,6 +203,74 @@ def test_layer_norm_gradient_against_differences():
         assert abs(num - float(dx[r, c])) <= 64 * U * 4 * 40 / h + 16 * h * h, (r, c, num, float(dx[r, c]))
 
 
+@gpu
+def test_layer_norm_pointers_of_any_alignment():
+    from erfnet_pytorch_amd import functional as hipf
+    for kind in TYPES.values():
+        x, gy, w, b = norm_case(21, 88, kind)
+        buf, bufg = (torch.zeros(21 * 88 + 9, dtype=kind, device=DEV) for _ in range(2))
+        for off in (1, 3, 8):
+            xs, gs = (t[off:off + 21 * 88].view(21, 88) for t in (buf, bufg))
+            xs.copy_(x), gs.copy_(gy)
+            args = [t.detach().requires_grad_() for t in (xs, w.to(DEV), b.to(DEV))]
+            y = hipf.layer_norm(*args)
+            check_norm((y.detach(), *torch.autograd.grad(y, args, gs)), x, gy, w, b, 1e-5, (kind, off))
+
+
+@gpu
+def test_layer_norm_beyond_32_bit_offsets():
+    """2^31 + 5120 elements: the last rows equal the same rows by themselves, bit for bit."""
+    from erfnet_pytorch_amd import functional as hipf
+    rows, c = (1 << 21) + 5, 1024
+    x = torch.zeros(rows, c, dtype=torch.bfloat16, device=DEV)
+    gy = torch.zeros_like(x)
+    tail, gtail, w, b = norm_case(6, c, torch.bfloat16)
+    x[-6:], gy[-6:] = tail.to(DEV), gtail.to(DEV)
+    w, b = w.to(DEV), b.to(DEV)
+    x.requires_grad_()
+    y = hipf.layer_norm(x, w, b)
+    dx, = torch.autograd.grad(y, x, gy)
+    part = tail.to(DEV).requires_grad_()
+    yp = hipf.layer_norm(part, w, b)
+    dxp, = torch.autograd.grad(yp, part, gtail.to(DEV))
+    assert torch.equal(y[-6:], yp) and torch.equal(dx[-6:], dxp)
+
+
+def test_layer_norm_module_on_the_cpu():
+    from erfnet_pytorch_amd.norm import LayerNorm
+    x, gy, w, b = norm_case(30, 12, torch.float32)
+    m = LayerNorm(12, dim=1)
+    with torch.no_grad():
+        m.weight.copy_(w), m.bias.copy_(b)
+    y = m(x.view(2, 5, 3, 12).permute(0, 3, 1, 2)).permute(0, 2, 3, 1).reshape(30, 12)
+    within(y.detach(), norm_reference(x, gy, w, b, 1e-5)[0][0], 1e-5, "module")
+    assert list(LayerNorm(4).state_dict()) == ["weight", "bias"] and not LayerNorm(4, affine=False).state_dict()
+    with pytest.raises(ValueError):
+        LayerNorm(4, dim=0)
+
+
+@gpu
+def test_layer_norm_module_between_blocks():
+    """In front of and behind a non_bottleneck_1d: NHWC in and out, gradients through both."""
+    from erfnet_pytorch_amd import erfnet_blocks
+    from erfnet_pytorch_amd.norm import LayerNorm
+    torch.manual_seed(3)
+    net = torch.nn.Sequential(LayerNorm(64, dim=1), erfnet_blocks.non_bottleneck_1d(64, 0.0, 1), LayerNorm(64, dim=1))
+    x = torch.randn(1, 64, 16, 24)
+    want = net(x)
+    g = torch.randn_like(want)
+    want_grads = torch.autograd.grad(want, list(p for p in net.parameters()), g, allow_unused=True)
+    net = net.to(DEV)
+    got = net(x.to(DEV))
+    got_grads = torch.autograd.grad(got, list(p for p in net.parameters()), g.to(DEV), allow_unused=True)
+    # convolutions of 64 x 3 products on both sides: 2e-4 of the largest value, as the blocks' own tests allow
+    assert (got.cpu() - want).abs().max() <= 2e-4 * want.abs().max()
+    for a, b_ in zip(got_grads, want_grads):
+        assert (a is None) == (b_ is None)
+        if a is not None:
+            assert (a.cpu() - b_).abs().max() <= 1e-3 * b_.abs().max().clamp(min=1e-6)
+
+
 # ================================================================================ log probabilities
 def lp_reference(x, target, k, ignore, g_lp=None, g_h=None, g_top=None):
     """Rows [n, V] in float64: results, the gradient, and the magnitudes its rounding error is proportional to."""
@@ -423,6 +491,42 @@ def test_log_probs_agree_with_cross_entropy():
     # p / count: both sides' relative error of p is below 256 u (1 + |t| + log S) with |t| < 32, log S < 4
     n = float((tg >= 0).sum())
     assert (a.grad - b.grad).abs().max() <= 2 * 256 * 37 * U / n
+
+
+@gpu
+def test_log_probs_beyond_32_bit_offsets():
+    """Rows and pixels whose last elements lie past 2^31, beside the same ones by themselves.  A row's segments depend on how
+    many rows there are, so its sums may differ in the last bits: 1e-5 of numbers below 20.  Pixels agree bit for bit."""
+    from erfnet_pytorch_amd import functional as hipf
+    v, rows = 65537, 32800
+    tail, t, _ = lp_case(3, v, torch.bfloat16, 4)
+    t = torch.tensor([5, v - 1, 7])
+    x = torch.zeros(rows, v, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = tail.to(DEV)
+    tg = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    tg[-3:] = t.to(DEV)
+    x.requires_grad_()
+    r = hipf.log_probs(x, tg, 4)
+    dx, = torch.autograd.grad(r.log_prob, x, torch.ones(rows, device=DEV))
+    part = tail.to(DEV).requires_grad_()
+    p = hipf.log_probs(part, t.to(DEV), 4)
+    dp, = torch.autograd.grad(p.log_prob, part, torch.ones(3, device=DEV))
+    assert (r.log_prob[-3:] - p.log_prob).abs().max() <= 2e-4 and torch.equal(r.top_indices[-3:], p.top_indices)
+    assert (dx[-3:].float() - dp.float()).abs().max() <= 2.0 ** -8
+    del x, dx, r
+    k, n = 66, 1 << 25
+    x = torch.zeros(1, k, n, dtype=torch.bfloat16, device=DEV)
+    x[:, :, -300:] = torch.randn(1, k, 300, generator=torch.Generator().manual_seed(2)).to(DEV)
+    tg = torch.full((1, n), 3, dtype=torch.int64, device=DEV)
+    x.requires_grad_()
+    r = hipf.log_probs(x, tg, 2, dim=1)
+    dx, = torch.autograd.grad(r.log_prob, x, torch.ones(1, n, device=DEV))
+    part = x.detach()[:, :, -8192:].contiguous().requires_grad_()
+    p = hipf.log_probs(part, tg[:, -8192:].contiguous(), 2, dim=1)
+    dp, = torch.autograd.grad(p.log_prob, part, torch.ones(1, 8192, device=DEV))
+    for a, b in ((r.log_prob[:, -8192:], p.log_prob), (r.entropy[:, -8192:], p.entropy), (dx[:, :, -8192:], dp),
+                 (r.top_indices[:, :, -8192:], p.top_indices)):
+        assert torch.equal(a, b)
 
 
 @gpu
@@ -729,6 +833,31 @@ def test_adamw_refuses_state_and_gradients_that_do_not_fit():
     assert torch.equal(p.detach(), kept)
 
 
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_beyond_32_bit_offsets(bits):
+    """2^31 + 700 bf16 parameters: the last blocks equal the same elements as a tensor of their own, bit for bit."""
+    from erfnet_pytorch_amd import optim
+    n, tail = (1 << 31) + 700, 1024 + 188
+    g = torch.Generator().manual_seed(6)
+    small, grad = torch.randn(tail, generator=g).bfloat16().to(DEV), torch.randn(tail, generator=g).bfloat16().to(DEV)
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device=DEV))
+    p.grad = torch.zeros_like(p)
+    with torch.no_grad():
+        p[-tail:] = small
+    p.grad[-tail:] = grad
+    q = torch.nn.Parameter(small.clone())
+    q.grad = grad.clone()
+    assert (n - tail) % 256 == 0
+    a, b = optim.AdamW([p], **HP, state_bits=bits), optim.AdamW([q], **HP, state_bits=bits)
+    for _ in range(2):
+        a.step(), b.step()
+    assert torch.equal(p.detach()[-tail:], q.detach())
+    for key, t in b.state[q].items():
+        if key != "step":
+            assert torch.equal(a.state[p][key][-t.numel():].view(torch.uint8), t.view(torch.uint8)), key
+
+
 # ================================================================================ together, streams, graphs
 def head_step(hipf, x, w, b, lin, t):
     """Norm, a linear head, log probabilities and an entropy bonus: the loss of one step."""
@@ -870,7 +999,11 @@ def test_adamw_refusals():
     for bad in (dict(lr=-1.0), dict(eps=-1.0), dict(weight_decay=-0.1), dict(betas=(1.0, 0.9)), dict(state_bits=16)):
         with pytest.raises(ValueError):
             optim.AdamW([p], **bad)
-    opt = optim.AdamW([p])
+    with pytest.raises(ValueError, match="twice"):
+        optim.AdamW([p, p])
+    with pytest.raises(ValueError, match="twice"):
+        optim.AdamW([("a", p), ("b", p)])
+    opt = optim.AdamW(iter([p]))
     p.grad = torch.ones(4)
     with pytest.raises(RuntimeError, match="GPU"):
         opt.step()
