@@ -164,7 +164,8 @@ struct LpList {
 };
 
 // ---------------------------------------------------------------------------------- rows: the class axis is the last
-template <int N, int U> __device__ __forceinline__ void lp_add_vectors(LpSums &r, const float (&v)[U][N])
+// Adds the values; gives back the largest.
+template <int N, int U> __device__ __forceinline__ float lp_add_vectors(LpSums &r, const float (&v)[U][N])
 {
     float high = v[0][0];
 #pragma unroll
@@ -176,19 +177,42 @@ template <int N, int U> __device__ __forceinline__ void lp_add_vectors(LpSums &r
     for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < N; ++i) lp_add(r, v[u][i]);
+    return high;
 }
 
+// The turns of a scan, 16 elements a thread each, in four quarters; the last has the turn that may lack some as well.
+struct LpTurns {
+    int step, turns, left;      // elements of all threads' vectors; whole turns; elements behind them
+    __device__ __forceinline__ LpTurns(int from, int to, int threads, int n, int u)
+    {
+        step = threads * n;
+        turns = (to - from) / (step * u);
+        left = to - from - turns * step * u;
+    }
+    __device__ __forceinline__ int begin(int quarter) const { return turns * quarter / 4; }
+};
+
 // What one thread does with its share of elements [from, to) of a row: 16 at a time in vectors `threads` apart, with the
-// next ones' loads in flight; the last turn, which may lack some, by itself.
-template <typename T>
-__device__ __forceinline__ LpSums lp_scan(const T *x, int from, int to, int me, int threads)
+// next ones' loads in flight; the last turn, which may lack some, by itself.  TOP: high[0..3] receive the quarters' maxima.
+template <typename T, bool TOP>
+__device__ __forceinline__ LpSums lp_scan(const T *x, int from, int to, int me, int threads, float (&high)[4])
 {
     constexpr int N = Vec16<T>::N, U = 16 / N;
     LpSums r = {LP_LOWEST, 0.0f, 0.0f};
-    const int step = threads * N, turns = (to - from) / (step * U);
+    const LpTurns plan(from, to, threads, N, U);
+    const int step = plan.step, turns = plan.turns;
     const T *at = x + from + me * N;
     u32x4 next[U];
     float v[U][N];
+    int quarter = 0, until = plan.begin(1);
+    high[0] = high[1] = high[2] = high[3] = -INFINITY;
+    auto turn_page = [&]() __attribute__((always_inline)) {     // (three times in all: the first quarter ends in high[0])
+        high[0] = high[1];
+        high[1] = high[2];
+        high[2] = high[3];
+        high[3] = -INFINITY;
+        until = plan.begin(++quarter + 1);
+    };
     auto fetch = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; ++u) next[u] = reinterpret_cast<const typename Vec16<T>::Raw *>(at + u * step)->v;
@@ -199,8 +223,13 @@ __device__ __forceinline__ LpSums lp_scan(const T *x, int from, int to, int me, 
 #pragma unroll
         for (int u = 0; u < U; ++u) Vec16<T>::unpack(next[u], v[u]);
         if (t + 1 < turns) fetch();
-        lp_add_vectors(r, v);
+        if (TOP)
+            while (quarter < 3 && t == until) turn_page();
+        const float top = lp_add_vectors(r, v);
+        if (TOP) high[3] = fmaxf(high[3], top);
     }
+    if (TOP)
+        while (quarter < 3) turn_page();
     const int c0 = from + turns * step * U + me * N;
     if (c0 < to) {
 #pragma unroll
@@ -211,29 +240,40 @@ __device__ __forceinline__ LpSums lp_scan(const T *x, int from, int to, int me, 
 #pragma unroll
             for (int i = 0; i < N; ++i) v[u][i] = c0 + u * step + i < to ? v[u][i] : -INFINITY;
         }
-        lp_add_vectors(r, v);
+        const float top = lp_add_vectors(r, v);
+        if (TOP) high[3] = fmaxf(high[3], top);
     }
     return r;
 }
 
-// The entries of this wave's threads that reach `bar`, into top.  `owner`: this thread may hold one.  A lane takes one
-// vector of one owner at a time, so that a few owners' long shares occupy the whole wave.
+// The entries of this wave's threads that reach `bar`, into top.  high: the threads' quarters' maxima; `spoilt`: they do not
+// show all there is.  A lane takes one vector of one quarter that reaches the bar at a time, so that the few there are
+// occupy the whole wave.  (Every such vector costs a cache line: by whole shares instead of quarters the second reading
+// fetched 28 % of a row of 100003 bf16 classes again, k = 8.)
 template <typename T>
-__device__ __forceinline__ void lp_collect(const T *x, int from, int to, int first, int threads, bool owner, unsigned bar,
-                                           int k, lp_lds8 *owners, LpList &top)
+__device__ __forceinline__ void lp_collect(const T *x, int from, int to, int first, int threads, const float (&high)[4],
+                                           bool spoilt, unsigned bar, int k, lp_lds8 *owners, LpList &top)
 {
-    constexpr int N = Vec16<T>::N;
-    const int lane = threadIdx.x & 63, step = threads * N;
-    const unsigned long long mask = __ballot(owner);
-    if (owner) {
-        const int at = __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
-        owners[at] = (unsigned char)lane;
+    constexpr int N = Vec16<T>::N, U = 16 / N;
+    const LpTurns plan(from, to, threads, N, U);
+    const int lane = threadIdx.x & 63, step = plan.step;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const bool some = plan.begin(j) < plan.begin(j + 1) || (j == 3 && plan.left > 0);
+        const bool owner = some && (spoilt || lp_key32(high[j]) >= bar);
+        const unsigned long long mask = __ballot(owner);
+        const int at = n + __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
+        if (owner) owners[at] = (unsigned char)(lane | j << 6);
+        n += __popcll(mask);
     }
-    const int turns = (to - from + step - 1) / step, n = __popcll(mask) * turns;
-    for (int q0 = 0; q0 < n; q0 += 64) {        // (the same number of turns for all lanes: the votes need them)
-        const int q = q0 + lane, o = q < n ? q / turns : 0;
-        const int c = from + (q - o * turns) * step + (first + owners[o]) * N;
-        const int left = q < n ? to - c : 0;
+    const int most = (plan.turns + 3) / 4 * U + (plan.left > 0 ? U : 0);       // vectors of a quarter, at most
+    for (int q0 = 0; q0 < n * most; q0 += 64) {     // (the same number of turns for all lanes: the votes need them)
+        const int q = q0 + lane, o = q / most, t = q - o * most;
+        const unsigned own = q < n * most ? owners[o] : 0u;
+        const int j = own >> 6, begin = plan.begin(j) * U, end = j == 3 ? begin + most : plan.begin(j + 1) * U;
+        const int c = from + (begin + t) * step + (first + (int)(own & 63u)) * N;
+        const int left = q < n * most && begin + t < end && c < to ? to - c : 0;
         float v[N];
         Vec16<T>::unpack(ld16(x + c, left), v);
         unsigned mine = 0;
@@ -297,7 +337,7 @@ __global__ __launch_bounds__(LP_BLOCK, 8) void lp_rows_kernel(const LpDesc d)
 {
     __shared__ unsigned long long buf[TOP ? 4 : 1][64];
     __shared__ unsigned high[TOP ? 4 : 1][64];
-    __shared__ unsigned char owners[TOP ? 4 : 1][64];
+    __shared__ unsigned char owners[TOP ? 4 : 1][256];
     __shared__ int counts[4];
     __shared__ LpSums sums[4];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -315,7 +355,8 @@ __global__ __launch_bounds__(LP_BLOCK, 8) void lp_rows_kernel(const LpDesc d)
         to = from + d.seg < d.V ? from + d.seg : d.V;
     }
     const T *x = (const T *)d.x + row * d.ld;
-    LpSums r = lp_scan<T>(x, from, to, me, GROUP);
+    float quarters[4];
+    LpSums r = lp_scan<T, TOP>(x, from, to, me, GROUP, quarters);
     LpList top;
     if (TOP) {
         top.buf = (lp_lds64 *)buf[wave];
@@ -331,8 +372,8 @@ __global__ __launch_bounds__(LP_BLOCK, 8) void lp_rows_kernel(const LpDesc d)
             for (int w = 1; w < 4; ++w) best = lp_merge(best, high[(wave + w) & 3][lane]);
         }
         const unsigned bar = (unsigned)__builtin_amdgcn_readlane((int)best, d.k - 1);
-        lp_collect<T>(x, from, to, GROUP == 256 ? wave * 64 : 0, GROUP, mine != 0u && (spoilt || mine >= bar), bar > 1u ? bar : 1u,
-                      d.k, (lp_lds8 *)owners[wave], top);
+        lp_collect<T>(x, from, to, GROUP == 256 ? wave * 64 : 0, GROUP, quarters, spoilt, bar > 1u ? bar : 1u, d.k,
+                      (lp_lds8 *)owners[wave], top);
     }
     r = lp_wave_join(r);
     if (GROUP == 64) {

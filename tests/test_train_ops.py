@@ -742,6 +742,22 @@ def test_adamw_groups_schedules_missing_gradients_and_flat_parameters():
 
 
 @gpu
+@pytest.mark.parametrize("kind", TYPES)
+def test_adamw_on_a_flat_buffer_equals_its_tensors(kind):
+    from erfnet_pytorch_amd import optim
+    ps, gs = adamw_tensors([40, 300, 1, 5000], TYPES[kind], seed=8)
+    flat = torch.nn.Parameter(torch.cat(ps).to(DEV))
+    params = [torch.nn.Parameter(p.to(DEV)) for p in ps]
+    a, b = optim.AdamW([flat], **HP), optim.AdamW(params, **HP)
+    for i in range(3):
+        flat.grad = torch.cat(gs[i]).to(DEV)
+        for p, g in zip(params, gs[i]):
+            p.grad = g.to(DEV)
+        a.step(), b.step()
+    assert torch.equal(flat.detach(), torch.cat([p.detach() for p in params]))
+
+
+@gpu
 def test_adamw_views_at_odd_offsets():
     """Parameters, gradients and moments that start at any element of a larger buffer, and what lies behind them stays."""
     from erfnet_pytorch_amd import optim
