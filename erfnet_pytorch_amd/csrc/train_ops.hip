@@ -168,10 +168,11 @@ bool lp_by_thread(long long outer, int V, long long inner, int k)
 #define LP_WAVE_BACKWARD 1024
 #define LP_BACKWARD_SEGMENT 8192
 
-// Forward, blocks per row: longer rows take whole blocks of at least 4096 classes, several to a row until there are
-// 4096 of them (2048 are resident), or 768 where every block also finds alternatives and a row's blocks have theirs to join.
-// 2047 x 100003 bf16, 1 / 2 / 3 / 5 blocks a row: 88 / 94 / 81 / 77 us without alternatives, 101 / 110 / 114 / 125 with 8;
-// 300 x 131072, 3 / 5 / 14 a row, with 8: 27 / 29 / 32.
+// Forward, blocks per row: longer rows take whole blocks of at least 4096 classes, several to a row until there are 8192 of
+// them (2048 are resident; more rounds even out what the memory channels give each block), or 4096 where every block also finds
+// alternatives and a row's blocks have theirs to join.  Behind a 512 MB write that empties the caches, 2047 x 100003 bf16,
+// 1 / 2 / 3 / 5 blocks a row: 146 / 150 / 138 / 131 us without alternatives, 155 / 158 / 149 / 149 with 8; 300 x 131072,
+// 3 / 7 / 14 / 32 a row, with 8: 44 / 47 / 45 / 59.
 struct LpPlan {
     bool wave;
     int splits, seg;
@@ -180,7 +181,7 @@ LpPlan lp_plan(long long rows, int V, int k)
 {
     LpPlan p = {V <= LP_WAVE_FORWARD, 1, V};
     if (p.wave) return p;
-    const long long want = ((k ? 768 : 4096) + rows - 1) / std::max<long long>(rows, 1);
+    const long long want = ((k ? 4096 : 8192) + rows - 1) / std::max<long long>(rows, 1);
     p.splits = (int)std::min<long long>(std::max<long long>(want, 1), (V + 4095) / 4096);
     p.seg = ((V + p.splits - 1) / p.splits + 4095) / 4096 * 4096;
     p.splits = (V + p.seg - 1) / p.seg;
