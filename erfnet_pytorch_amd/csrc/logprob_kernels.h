@@ -454,21 +454,23 @@ __device__ __forceinline__ float lp_grad(float x, float m, float log_s, float G,
     return -p * (G + gh * (fmaxf(lp, LP_FLOOR) + H));
 }
 
-// GROUP threads take a segment of a row (GROUP = 64: the whole row).
+// GROUP threads take a segment of a row (GROUP = 64: the whole row).  The backward kernels walk from the last row to the
+// first: what forward read last is what the 256 MB cache still has (6 x 20 x 512 x 1024 fp32: 129 -> 125 us).
 template <typename T, int GROUP>
 __global__ __launch_bounds__(LP_BLOCK) void lp_rows_bwd_kernel(const LpDesc d)
 {
     constexpr int N = Vec16<T>::N;
     const int lane = threadIdx.x & 63;
+    const unsigned block = gridDim.x - 1 - blockIdx.x;
     long long row;
     int me, from = 0, to = d.V;
     if (GROUP == 64) {
-        row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+        row = (long long)block * 4 + (threadIdx.x >> 6);
         me = lane;
     } else {
-        row = blockIdx.x / d.splits;
+        row = block / d.splits;
         me = threadIdx.x;
-        from = (int)(blockIdx.x - row * d.splits) * d.seg;
+        from = (int)(block - row * d.splits) * d.seg;
         to = from + d.seg < d.V ? from + d.seg : d.V;
     }
     const bool live = row < d.rows;
@@ -523,7 +525,7 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_short_rows_bwd_kernel(const LpDes
 {
     __shared__ float m[LP_SHORT_ROWS], log_s[LP_SHORT_ROWS], G[LP_SHORT_ROWS], gh[LP_SHORT_ROWS], H[LP_SHORT_ROWS], glp[LP_SHORT_ROWS];
     __shared__ int target[LP_SHORT_ROWS];
-    const long long row0 = (long long)blockIdx.x * LP_SHORT_ROWS;
+    const long long row0 = (long long)(gridDim.x - 1 - blockIdx.x) * LP_SHORT_ROWS;
     const int rows = d.rows - row0 < LP_SHORT_ROWS ? (int)(d.rows - row0) : LP_SHORT_ROWS, V = d.V, k = d.g_top ? d.k : 0;
     // four threads add up a row's upstream gradients
     const int mine = threadIdx.x >> 2, part = threadIdx.x & 3;
@@ -642,7 +644,7 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_pixels_kernel(const LpDesc d)
 template <typename T, int K>
 __global__ __launch_bounds__(LP_BLOCK) void lp_pixels_bwd_kernel(const LpDesc d)
 {
-    const long long p = (long long)blockIdx.x * LP_BLOCK + threadIdx.x;
+    const long long p = (long long)(gridDim.x - 1 - blockIdx.x) * LP_BLOCK + threadIdx.x;
     if (p >= d.rows) return;
     const long long n = p / d.inner, q = p - n * d.inner;
     const T *x = (const T *)d.x + n * d.group + q;

@@ -138,7 +138,8 @@ __global__ __launch_bounds__(LANES ? NORM_BLOCK : 1024) void norm_fwd_kernel(con
     }
 }
 
-// Backward, the same walk.  Every thread keeps the weight's and bias's gradient of its own channels in registers over
+// Backward, the same walk, from the last row to the first: what was read and written last is what the 256 MB cache
+// still has (8191 x 8192 bf16: 93.9 -> 92.5 us).  Every thread keeps the weight's and bias's gradient of its own channels in registers over
 // all rows it meets; the block's sums go to partial, and norm_grad_sum_kernel adds the blocks in order.
 // THREADS: most threads of a block kernel (0: wave kernel).  1024 of them have 128 registers each, which hold the sums
 // but neither the weight nor the next row's loads: AHEAD is off there.
@@ -157,7 +158,8 @@ __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kerne
     long long row = (long long)blockIdx.x * rows_per_block + (BLOCK ? 0 : threadIdx.x / (BLOCK ? 1 : LANES));
     u32x4 nx[R], ng[R];
     float nmean = 0.0f, nrstd = 0.0f;
-    auto fetch = [&](long long at) __attribute__((always_inline)) {
+    auto fetch = [&](long long row) __attribute__((always_inline)) {
+        const long long at = d.rows - 1 - row;
         norm_load<T, R, EVEN>(nx, d, d.x, at, me, threads);
         norm_load<T, R, EVEN>(ng, d, d.gy, at, me, threads);
         nmean = d.mean[at];
@@ -208,7 +210,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kerne
         }
         s0 *= inv_c;
         s1 *= inv_c;
-        T *dx = (T *)d.y + row * C;
+        T *dx = (T *)d.y + (d.rows - 1 - row) * C;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int c = (r * threads + me) * N;
