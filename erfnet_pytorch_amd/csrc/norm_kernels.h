@@ -248,23 +248,26 @@ __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kerne
     for (int j = threadIdx.x; j < 2 * C; j += NORM_BLOCK) out[j] = acc[j] + acc[2 * C + j] + acc[4 * C + j] + acc[6 * C + j];
 }
 
-// dw[c], db[c] = sum over blocks of partial[block][0 / 1][c]: 16 columns x 64 rows of threads a block, each row's blocks in
-// a fixed order, then the 64 rows in order.
+// dw[c], db[c] = sum over blocks of partial[block][0 / 1][c]: COLS columns x 1024 / COLS rows of threads a block, each row's
+// blocks in a fixed order, then the rows in order.  Few columns want many rows (there are few blocks to hide the latency of
+// a row's loads), many columns want whole cache lines.
+template <int COLS>
 __global__ __launch_bounds__(1024) void norm_grad_sum_kernel(const float *partial, int nblocks, int C, float *dw, float *db)
 {
-    __shared__ float red[64][17];
-    const int col = threadIdx.x & 15, part = threadIdx.x >> 4, j = blockIdx.x * 16 + col;
+    constexpr int ROWS = 1024 / COLS;
+    __shared__ float red[ROWS][COLS + 1];
+    const int col = threadIdx.x % COLS, part = threadIdx.x / COLS, j = blockIdx.x * COLS + col;
     float s = 0.0f;
     if (j < 2 * C) {
 #pragma unroll 8
-        for (int i = part; i < nblocks; i += 64) s += partial[(long long)i * 2 * C + j];
+        for (int i = part; i < nblocks; i += ROWS) s += partial[(long long)i * 2 * C + j];
     }
     red[part][col] = s;
     __syncthreads();
     if (part == 0 && j < 2 * C) {
         float t = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) t += red[i][col];
+        for (int i = 0; i < ROWS; ++i) t += red[i][col];
         if (j < C) { if (dw) dw[j] = t; }
         else if (db) db[j - C] = t;
     }

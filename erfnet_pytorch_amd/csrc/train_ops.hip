@@ -78,6 +78,10 @@ int norm_blocks(const NormPlan &p, long long rows, int threads, int turns)
 #define NORM_FWD_BLOCKS(p, rows) norm_blocks(p, rows, 2048, 1)
 #define NORM_BWD_BLOCKS(p, rows) norm_blocks(p, rows, 1024, 8)
 
+// (partial sums of wide rows, us with 16 / 64 columns a block: C = 2048 12.6 / 11.8, 4096 11.9 / 8.1, 8192 13.3 / 7.3; 16 below,
+// where 64 leave most compute units without a block)
+#define NORM_SUM_WIDE 2048
+
 int norm_check(const char *what, const void *x, const void *y, long long rows, int C, float eps)
 {
     if (rows < 0) return fail("%s: negative row count", what);
@@ -141,7 +145,9 @@ int norm_backward(const void *x, const float *w, const float *mean, const float 
         LAUNCHED("norm_bwd_kernel");
     }
     if (params) {
-        norm_grad_sum_kernel<<<(2 * C + 15) / 16, 1024, 0, st>>>((const float *)ws, blocks, C, dw, db);   // (no rows: zeros)
+        // (no rows: zeros)
+        if (C >= NORM_SUM_WIDE) norm_grad_sum_kernel<64><<<(2 * C + 63) / 64, 1024, 0, st>>>((const float *)ws, blocks, C, dw, db);
+        else norm_grad_sum_kernel<16><<<(2 * C + 15) / 16, 1024, 0, st>>>((const float *)ws, blocks, C, dw, db);
         LAUNCHED("norm_grad_sum_kernel");
     }
     return 0;

@@ -224,7 +224,6 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p][k] = given[k].detach().to(p.device, copy=True).contiguous()
                 self.state[p]["step"] = torch.tensor(float(given["step"]))
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
@@ -240,7 +239,8 @@ class AdamW(torch.optim.Optimizer):
                     float(group["eps"]), float(group["weight_decay"]))
             first = host.adamw_step(*args)
             if first:                   # parameters that have their first gradient: nothing has been launched yet
-                for p in first:
-                    self.state[p].update(self._new_state(p))
+                with torch.no_grad():
+                    for p in first:
+                        self.state[p].update(self._new_state(p))
                 host.adamw_step(*args)
         return loss
