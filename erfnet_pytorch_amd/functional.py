@@ -1303,6 +1303,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, dim=-1):
     if not eps >= 0:
         raise ValueError(f"layer_norm: eps must not be negative (got {eps})")
     _need_gpu("layer_norm", x, weight, bias)
+    _materialize_logits(x)
     return _lib.host().layer_norm(x, weight, bias, float(eps), axis != nd - 1)
 
 

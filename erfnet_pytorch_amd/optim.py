@@ -221,7 +221,9 @@ class AdamW(torch.optim.Optimizer):
             if i in state_dict["state"]:
                 given = state_dict["state"][i]
                 for k in want:
-                    self.state[p][k] = given[k].detach().to(p.device, copy=True).contiguous()
+                    # (torch.optim.AdamW keeps a bf16 parameter's moments in bf16)
+                    dtype = given[k].dtype if given[k].dtype == torch.float8_e4m3fn else torch.float32
+                    self.state[p][k] = given[k].detach().to(p.device, dtype, copy=True).contiguous()
                 self.state[p]["step"] = torch.tensor(float(given["step"]))
 
     def step(self, closure=None):

@@ -531,6 +531,47 @@ def test_log_probs_beyond_32_bit_offsets():
 
 @gpu
 @pytest.mark.parametrize("op", ["layer_norm", "log_probs"])
+def test_deferred_logits_of_the_network(op):
+    """net_classification.Net hands out logits whose kernel has not run; these two read the memory itself, so they run it
+    first.  Same numbers and parameter gradients as with logits that are written at once."""
+    from erfnet_pytorch_amd import functional as hipf, net_classification
+    torch.manual_seed(0)
+    net = net_classification.Net(softmax_classes=20).to(DEV).train()
+    x = torch.rand(1, 3, 64, 128, generator=torch.Generator().manual_seed(1)).to(DEV)
+    t = torch.randint(-1, 20, (1, 64, 128), generator=torch.Generator().manual_seed(2)).to(DEV)
+    results = []
+    for lazy in (False, True):
+        old = hipf.set_lazy_logits(lazy)
+        try:
+            logits = net(x)
+            logits = logits[0] if isinstance(logits, (tuple, list)) else logits
+            if op == "layer_norm":
+                out = hipf.layer_norm(logits, dim=1)
+                loss = (out * out * t.unsqueeze(1)).sum()
+            else:
+                out = hipf.log_probs(logits, t, 2, 1)
+                loss = -(out.log_prob + 0.1 * out.entropy).mean()
+                out = out.log_prob
+            w = net.encoder.initial_block.conv.weight
+            results.append((out.detach(), torch.autograd.grad(loss, w)[0]))
+        finally:
+            hipf.set_lazy_logits(old)
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    assert results[0][0].abs().max() > 0 and results[0][1].abs().max() > 0
+
+
+@gpu
+def test_operands_on_two_devices_are_refused():
+    from erfnet_pytorch_amd import functional as hipf
+    x = torch.zeros(4, 8, device=DEV)
+    with pytest.raises(RuntimeError, match="cpu"):
+        hipf.log_probs(x, torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="cpu"):
+        hipf.layer_norm(x, torch.ones(8))
+
+
+@gpu
+@pytest.mark.parametrize("op", ["layer_norm", "log_probs"])
 def test_gradients_are_not_differentiable(op):
     from erfnet_pytorch_amd import functional as hipf
     x = torch.randn(4, 32, generator=torch.Generator().manual_seed(1)).to(DEV).requires_grad_()
@@ -651,6 +692,27 @@ def test_adamw_follows_torch_and_shares_its_state_dict(wd):
         a.step(), b.step()
     for p, q in zip(mine, theirs):
         assert (p - q).abs().max() <= 10 * (8 * U * p.abs().max() + 64 * U * HP["lr"] * 10)
+
+
+@gpu
+def test_adamw_takes_the_state_of_torchs_bf16_optimiser():
+    """torch.optim.AdamW holds a bf16 parameter's moments in bf16; they are widened, and the next step is the formula's."""
+    from erfnet_pytorch_amd import optim
+    (p0,), gs = adamw_tensors([500], torch.bfloat16, seed=12)
+    theirs = torch.nn.Parameter(p0.to(DEV))
+    b = torch.optim.AdamW([theirs], **HP, foreach=False)
+    theirs.grad = gs[0][0].to(DEV)
+    b.step()
+    mine = torch.nn.Parameter(theirs.detach().clone())
+    a = optim.AdamW([mine], **HP)
+    a.load_state_dict(b.state_dict())
+    st = {k: t.cpu() for k, t in a.state[mine].items()}
+    assert st["exp_avg"].dtype == st["exp_avg_sq"].dtype == torch.float32
+    mine.grad = gs[1][0].to(DEV)
+    before = mine.detach().cpu().clone()
+    a.step()
+    ref, _, _, upd = adamw_reference(before, gs[1][0], st["exp_avg"].double(), st["exp_avg_sq"].double(), 2, HP)
+    within(mine.detach(), ref, 2.0 ** -8 * ref.abs() + 4 * U * before.double().abs() + 25 * U * upd, "step 2")
 
 
 @gpu
@@ -920,8 +982,7 @@ def test_norm_and_log_probs_on_another_stream_and_in_a_graph():
     up = [torch.randn(n, generator=g).to(DEV) for n in ((3,), (3,), (3, 3))]
 
     def work(x, wl, bl):
-        # the framework's own kernels only: a captured library product or sum may record memory-set nodes, and torch's own
-        # layer_norm - product - log_softmax chain in this place gives wrong numbers on a replay
+        # the framework's own kernels only (a captured library product or sum may record memory-set nodes)
         r = hipf.log_probs(hipf.layer_norm(x, wl, bl), t, 3)
         dw, db = torch.autograd.grad([r.log_prob, r.entropy, r.top_log_probs], (wl, bl), up)
         return [r.log_prob.detach(), r.entropy.detach(), r.top_indices, dw, db]
@@ -949,14 +1010,14 @@ def test_norm_and_log_probs_on_another_stream_and_in_a_graph():
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=side):
             out = work(static, wl, bl)
-        graphs.append((graph, static, out))
+        graphs.append((graph, static, out, wl, bl))       # (the graph reads the leaves' memory: they have to live as long)
     for i in (1, 2, 3, 0):
-        for k, (graph, static, out) in enumerate(graphs):
+        for k, (graph, static, out, _, _) in enumerate(graphs):
             static.copy_(xs[(i + k) % 4])
             graph.replay()
         work(xs[0], *leaves())
         torch.cuda.synchronize()
-        for k, (graph, static, out) in enumerate(graphs):
+        for k, (graph, static, out, _, _) in enumerate(graphs):
             for a, c in zip(out, eager[(i + k) % 4]):
                 assert torch.equal(a, c), (i, k)
 
