@@ -565,6 +565,7 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_short_rows_bwd_kernel(const LpDes
         if (log_s[r] == -INFINITY) continue;
         const long long at = (row0 + r) * d.k + j;
         const int c = (int)d.top_idx[at];
+        if (c < 0 || c >= V) continue;          // (not one of forward's)
         const float g = lp_grad(Vec16<T>::get(x + r * d.ld + c), m[r], log_s[r], G[r], gh[r], H[r]) + d.g_top[at];
         Vec16<T>::put(dx + (long long)r * V + c, c == target[r] ? g + glp[r] : g);
     }

@@ -23,10 +23,13 @@ class LayerNorm(nn.Module):
         self.bias = nn.Parameter(torch.zeros(num_channels)) if affine and bias else None
 
     def forward(self, input):
+        if input.dim() < (2 if self.dim == 1 else 1) or input.shape[self.dim] != self.num_channels:
+            raise ValueError(f"LayerNorm: {self.num_channels} channels on axis {self.dim} of {tuple(input.shape)}")
         if input.is_cuda:
             return hipf.layer_norm(input, self.weight, self.bias, self.eps, self.dim)
         x = input.movedim(self.dim, -1)
-        y = torch.nn.functional.layer_norm(x.float(), (self.num_channels,), self.weight, self.bias, self.eps)
+        w, b = (None if p is None else p.float() for p in (self.weight, self.bias))
+        y = torch.nn.functional.layer_norm(x.float(), (self.num_channels,), w, b, self.eps)
         return y.to(input.dtype).movedim(-1, self.dim)
 
     def extra_repr(self):

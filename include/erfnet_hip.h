@@ -428,6 +428,7 @@ int erf_ema_update(int count, float *const *target, const float *const *source, 
                    double discount, void *stream);
 
 /* AdamW (weight decay taken off the parameter, not added to the gradient) over many tensors; arguments as erf_adam_step.
+ * The tensors must not overlap: their updates run side by side.  A stream that is being captured is refused.
  * erf_adamw8_step keeps the moments in 8 bits: exp_avg and the square ROOT of exp_avg_sq as float8 e4m3 codes (numel bytes
  * each) with one fp32 scale per 256 consecutive elements of a tensor (ceil(numel / 256) scales; value = code * scale,
  * scale = the block's largest magnitude / 448; all zeros is the state before the first step).  The update itself uses the

@@ -247,6 +247,16 @@ def test_layer_norm_module_on_the_cpu():
     assert list(LayerNorm(4).state_dict()) == ["weight", "bias"] and not LayerNorm(4, affine=False).state_dict()
     with pytest.raises(ValueError):
         LayerNorm(4, dim=0)
+    with pytest.raises(ValueError, match="4 channels"):
+        LayerNorm(4, affine=False)(torch.zeros(3, 5))
+    with pytest.raises(ValueError, match="4 channels"):
+        LayerNorm(4, dim=1)(torch.zeros(4))
+    # one rounding of the result to bf16 on top of fp32's
+    y = m.bfloat16()(x.view(2, 5, 3, 12).permute(0, 3, 1, 2).bfloat16())
+    x16, w16, b16 = x.bfloat16(), w.bfloat16(), b.bfloat16()
+    want = norm_reference(x16, gy, w16, b16, 1e-5)[0][0]
+    got = y.detach().permute(0, 2, 3, 1).reshape(30, 12)
+    assert y.dtype == torch.bfloat16 and ((got.double() - want).abs() <= want.abs() * 2.0 ** -8 + 1e-5).all()
 
 
 @gpu
@@ -834,6 +844,25 @@ def test_adamw_views_at_odd_offsets():
         a, b = optim.AdamW([p], **HP, state_bits=bits), optim.AdamW([q], **HP, state_bits=bits)
         a.step(), b.step()
         assert torch.equal(p, q) and torch.equal(base[:3], keep[:3]) and torch.equal(base[1003:], keep[1003:])
+
+
+@gpu
+def test_adamw_refuses_parameters_that_share_memory():
+    from erfnet_pytorch_amd import optim
+    buf = torch.zeros(100, device=DEV)
+    apart = [torch.nn.Parameter(buf[:40]), torch.nn.Parameter(buf[40:]), torch.nn.Parameter(buf[:0])]
+    optim.AdamW(apart)
+    shared = apart + [torch.nn.Parameter(buf[39:41])]
+    with pytest.raises(ValueError, match="share memory"):
+        optim.AdamW(shared)
+    late = [torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(4))]
+    opt = optim.AdamW(late)
+    for p in late:
+        p.data = buf[:4]
+        p.grad = torch.ones(4, device=DEV)
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step()
+    assert not opt.state and not buf.any()
 
 
 @gpu
