@@ -86,7 +86,7 @@ __device__ __forceinline__ void lp_join(LpSums &r, LpSums o)
 // The scan itself looks for no alternatives: it leaves every thread with its maximum, and the k-th largest of those is a
 // bar that at least k entries reach.  Only threads whose maximum reaches it can hold an alternative, about k of them, and only
 // their entries are read again.  (Filtering entries against a running bar inside the scan took 240 us for 2047 rows of
-// 100003 bf16 classes, k = 8; the scan alone takes 100.)
+// 100003 bf16 classes, k = 8, the bar 114 when it came in its place, the scan without alternatives 82.)
 //
 // Sorting networks over the 64 lanes, larger values in lower lanes.
 template <int O> __device__ __forceinline__ unsigned lp_xor(unsigned v) { return wave_xor<O>(v); }

@@ -50,7 +50,8 @@ typedef struct {
  * mismatch (struct layouts are part of the ABI: revision 101 added erf_bn_t::num_batches_tracked and
  * changed erf_nb1d_block_t's member types, 102 added ERF_OPT_X3_ROLL and the capture rule of
  * erf_cross_entropy_forward_static, 103 added erf_nb1d_block_t::sign_bits / sign_bits_written and
- * erf_nb1d_backward_bits, 104 the erf_batch_* calls, 105 ERF_OPT_POOL_FUSE). */
+ * erf_nb1d_backward_bits, 104 the erf_batch_* calls, 105 ERF_OPT_POOL_FUSE, 106 layer norm, log
+ * probabilities and AdamW). */
 #define ERF_ABI_VERSION 106
 int erf_version(void);
 const char *erf_last_error(void);
