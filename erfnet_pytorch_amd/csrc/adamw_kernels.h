@@ -17,14 +17,16 @@
 #include "vec16.h"
 #include "wave.h"
 
+// (two rounds a wave: 4 take 105 registers with 8-bit moments and leave 4 waves a SIMD; bf16, 64 / 512 MB 24.0 / 146 us, 22.9 /
+// 138 with 2; with fp32 moments within 2 %)
 #define ADAMW_BLOCK 256
 #define ADAMW_SCALE_BLOCK 256
-#define ADAMW_ROUNDS 4
+#define ADAMW_ROUNDS 2
 #define ADAMW_CHUNK (ADAMW_BLOCK * 4 * ADAMW_ROUNDS)
 #define ADAMW_TINY 7.8886090522101181e-31f      // 2^-100: 448 / x stays finite above it; blocks below are stored as zeros
 
 struct AdamwScalars {
-    float b1, ob1, b2, ob2, keep, step, root_c2, eps;           // ob = 1 - b, keep = 1 - lr wd, step = lr / c1
+    float b1, ob1, b2, ob2, keep, step, inv_root_c2, eps;       // ob = 1 - b, keep = 1 - lr wd, step = lr / c1
 };
 // The pointers of one launch's tensors, as many as 4 KB of kernel arguments hold.
 template <int BITS> struct AdamwDesc {
@@ -50,69 +52,88 @@ template <> struct AdamwDesc<8> {
 };
 static_assert(sizeof(AdamwDesc<32>) <= 4096 && sizeof(AdamwDesc<8>) <= 4096, "kernel arguments");
 
+// sqrt to one unit in the last place: the instruction has that, but takes subnormal numbers for zero.
+__device__ __forceinline__ float adamw_root(float v)
+{
+    const bool small = v < 1.2621774483536189e-29f;             // 2^-96
+    const float r = __builtin_amdgcn_sqrtf(v * (small ? 4294967296.0f : 1.0f));
+    return r * (small ? 1.52587890625e-05f : 1.0f);             // 2^32, 2^-16
+}
+// b1 m + (1 - b1) g, each product rounded: a fused product would be nearer by half a unit, but a moment on the border between
+// two 8-bit codes would then fall to another one than in an update written with torch's operations, and a block whose largest
+// moment does so has another scale one step later (one block of 1.5 million; none with the same roundings here and in encode).
+__device__ __forceinline__ float adamw_mean(const AdamwScalars &d, float m, float g)
+{
+#pragma clang fp contract(off)
+    const float a = d.b1 * m, b = d.ob1 * g;
+    return a + b;
+}
+// The quotient is a product with a reciprocal to one unit in the last place.  (With exact roots and quotients and a
+// maximum of its own for every scale the 8-bit step took 85 vector instructions an element, and those bound it: bf16
+// parameters, 720 MB, 325 us, 198 so; fp32 232 and 180; with fp32 moments memory binds either way.)
 __device__ __forceinline__ float adamw_update(const AdamwScalars &d, float p, float g, float &m, float &v, float &root)
 {
-    m = d.b1 * m + d.ob1 * g;
+    m = adamw_mean(d, m, g);
     v = d.b2 * v + d.ob2 * (g * g);
-    root = sqrtf(v);
-    return p * d.keep - d.step * m / (root / d.root_c2 + d.eps);
+    root = adamw_root(v);
+    return p * d.keep - d.step * m * __builtin_amdgcn_rcpf(root * d.inv_root_c2 + d.eps);
 }
 
 // four consecutive elements, the first `left` of them there
 template <typename T> struct AdamwQuad;
 template <> struct AdamwQuad<float> {
     struct __attribute__((packed, aligned(4))) Raw { f32x4 v; };
-    static __device__ __forceinline__ f32x4 load(const void *p, long long i, int left)
+    template <bool STREAM> static __device__ __forceinline__ f32x4 load(const void *p, long long i, int left)
     {
         f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
         const float *q = (const float *)p + i;
-        if (left >= 4) r = reinterpret_cast<const Raw *>(q)->v;
+        if (left >= 4) r = ld_vec<STREAM>(reinterpret_cast<const Raw *>(q));
         else
             for (int j = 0; j < 3; ++j) if (j < left) r[j] = q[j];
         return r;
     }
-    static __device__ __forceinline__ void store(void *p, long long i, int left, f32x4 r)
+    template <bool STREAM> static __device__ __forceinline__ void store(void *p, long long i, int left, f32x4 r)
     {
         float *q = (float *)p + i;
-        if (left >= 4) reinterpret_cast<Raw *>(q)->v = r;
+        if (left >= 4) st_vec<STREAM>(reinterpret_cast<Raw *>(q), r);
         else
             for (int j = 0; j < 3; ++j) if (j < left) q[j] = r[j];
     }
 };
 template <> struct AdamwQuad<bf16_t> {
     struct __attribute__((packed, aligned(2))) Raw { u32x2 v; };
-    static __device__ __forceinline__ f32x4 load(const void *p, long long i, int left)
+    template <bool STREAM> static __device__ __forceinline__ f32x4 load(const void *p, long long i, int left)
     {
         f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
         const bf16_t *q = (const bf16_t *)p + i;
-        if (left >= 4) r = unpack_bf16x4(reinterpret_cast<const Raw *>(q)->v);
+        if (left >= 4) r = unpack_bf16x4(ld_vec<STREAM>(reinterpret_cast<const Raw *>(q)));
         else
             for (int j = 0; j < 3; ++j) if (j < left) r[j] = bf16_to_f32(q[j]);
         return r;
     }
-    static __device__ __forceinline__ void store(void *p, long long i, int left, f32x4 r)
+    template <bool STREAM> static __device__ __forceinline__ void store(void *p, long long i, int left, f32x4 r)
     {
         bf16_t *q = (bf16_t *)p + i;
-        if (left >= 4) reinterpret_cast<Raw *>(q)->v = pack_bf16x4(r);
+        if (left >= 4) st_vec<STREAM>(reinterpret_cast<Raw *>(q), pack_bf16x4(r));
         else
             for (int j = 0; j < 3; ++j) if (j < left) q[j] = f32_to_bf16(r[j]);
     }
 };
 struct AdamwCodes {
     struct __attribute__((packed, aligned(1))) Raw { unsigned v; };
-    static __device__ __forceinline__ unsigned load(const void *p, long long i, int left)
+    template <bool STREAM> static __device__ __forceinline__ unsigned load(const void *p, long long i, int left)
     {
         const unsigned char *q = (const unsigned char *)p + i;
         unsigned r = 0;
-        if (left >= 4) r = reinterpret_cast<const Raw *>(q)->v;
+        if (left >= 4) r = ld_vec<STREAM>(reinterpret_cast<const Raw *>(q));
         else
             for (int j = 0; j < 3; ++j) if (j < left) r |= (unsigned)q[j] << (8 * j);
         return r;
     }
-    static __device__ __forceinline__ void store(void *p, long long i, int left, unsigned r)
+    template <bool STREAM> static __device__ __forceinline__ void store(void *p, long long i, int left, unsigned r)
     {
         unsigned char *q = (unsigned char *)p + i;
-        if (left >= 4) reinterpret_cast<Raw *>(q)->v = r;
+        if (left >= 4) st_vec<STREAM>(reinterpret_cast<Raw *>(q), r);
         else
             for (int j = 0; j < 3; ++j) if (j < left) q[j] = (unsigned char)(r >> (8 * j));
     }
@@ -121,25 +142,42 @@ struct AdamwCodes {
         const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)r, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)r, true);
         return (f32x4){a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale};
     }
-    // codes of x at the wave's own scale (all 64 lanes take part); ROOT: x >= 0 and nonzero stays nonzero
-    template <bool ROOT> static __device__ __forceinline__ unsigned encode(f32x4 x, float &scale)
+    // As bits, magnitudes have the order of the values, infinity and NaN above them all: one maximum finds the scale and
+    // says whether there are any, one minimum whether a root would round to zero; only then a wave goes element by element.
+    static constexpr unsigned INF = 0x7f800000u;
+    static __device__ __forceinline__ unsigned bits(float x) { return __builtin_bit_cast(unsigned, x) & 0x7fffffffu; }
+    static __device__ __forceinline__ unsigned most(f32x4 x, unsigned below = ~0u)      // of this lane's, below `below`
     {
-        float top = 0.0f;
+        unsigned top = 0u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float a = fabsf(x[j]);
-            top = fmaxf(top, a < INFINITY ? a : 0.0f);
-        }
-        top = wave_max(top);
-        const bool some = top >= ADAMW_TINY;
-        const float inv = some ? 448.0f / top : 0.0f;
-        scale = some ? top / 448.0f : 0.0f;
+        for (int j = 0; j < 4; ++j) top = bits(x[j]) > top && bits(x[j]) < below ? bits(x[j]) : top;
+        return top;
+    }
+    // codes of x, whose largest magnitude over the wave is `top` (all 64 lanes take part); ROOT: x >= 0 and nonzero stays nonzero
+    template <bool ROOT> static __device__ __forceinline__ unsigned encode(f32x4 x, unsigned top, float &scale)
+    {
+        const bool odd = top >= INF;
+        if (odd) top = __builtin_bit_cast(unsigned, wave_max(__builtin_bit_cast(float, most(x, INF))));
+        const float high = __builtin_bit_cast(float, top);
+        const bool some = high >= ADAMW_TINY;
+        scale = some ? high * (1.0f / 448.0f) : 0.0f;
+        // 448 (1 / high), as torch divides; the reciprocal, of high / 4 because that is never subnormal, with its remainder
+        // added back
+        const float q = 0.25f * high, r0 = __builtin_amdgcn_rcpf(q);
+        const float inv = some ? 112.0f * __builtin_fmaf(__builtin_fmaf(-q, r0, 1.0f), r0, r0) : 0.0f;
         float y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            y[j] = x[j] * inv;
-            if (ROOT && some && x[j] > 0.0f) y[j] = fmaxf(y[j], 0.001953125f);     // 2^-9, the least code above zero
-            if (!(fabsf(x[j]) < INFINITY)) y[j] = __builtin_nanf("");
+        for (int j = 0; j < 4; ++j) y[j] = x[j] * inv;
+        if (ROOT) {
+            constexpr float code = 0.001953125f;                // 2^-9, the least above zero
+            if (some && __any(fminf(fminf(y[0], y[1]), fminf(y[2], y[3])) < code)) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = bits(x[j]) ? fmaxf(y[j], code) : 0.0f;
+            }
+        }
+        if (odd) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = bits(x[j]) >= INF ? __builtin_nanf("") : y[j];
         }
         int r = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
         r = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], r, true);
@@ -148,8 +186,9 @@ struct AdamwCodes {
 };
 
 // A wave's `ADAMW_ROUNDS` blocks of 256 elements, the first at `base`, blocks ADAMW_BLOCK * 4 elements apart; all loads go
-// out before the first result is needed.  FULL: every element is there.
-template <typename T, int BITS, bool FULL>
+// out before the first result is needed.  FULL: every element is there.  STREAM: reads, and the moments' writes, past the caches
+// (ADAMW_STREAM in train_ops.hip).
+template <typename T, int BITS, bool FULL, bool STREAM>
 __device__ __forceinline__ void adamw_chunk(const AdamwDesc<BITS> &d, int t, long long n, long long base)
 {
     const int lane = threadIdx.x & 63;
@@ -160,17 +199,18 @@ __device__ __forceinline__ void adamw_chunk(const AdamwDesc<BITS> &d, int t, lon
     for (int r = 0; r < ADAMW_ROUNDS; ++r) {
         const long long at = base + (long long)r * ADAMW_BLOCK * 4, i = at + lane * 4;
         const int left = FULL ? 4 : n - i >= 4 ? 4 : n - i > 0 ? (int)(n - i) : 0;
-        p[r] = AdamwQuad<T>::load(d.p[t], i, left);
-        g[r] = AdamwQuad<T>::load(d.g[t], i, left);
+        p[r] = AdamwQuad<T>::template load<STREAM>(d.p[t], i, left);
+        g[r] = AdamwQuad<T>::template load<STREAM>(d.g[t], i, left);
         if constexpr (BITS == 32) {
-            m[r] = AdamwQuad<float>::load(d.m[t], i, left);
-            v[r] = AdamwQuad<float>::load(d.v[t], i, left);
+            m[r] = AdamwQuad<float>::load<STREAM>(d.m[t], i, left);
+            v[r] = AdamwQuad<float>::load<STREAM>(d.v[t], i, left);
         } else {
-            cm[r] = AdamwCodes::load(d.m[t], i, left);
-            cr[r] = AdamwCodes::load(d.r[t], i, left);
+            cm[r] = AdamwCodes::load<STREAM>(d.m[t], i, left);
+            cr[r] = AdamwCodes::load<STREAM>(d.r[t], i, left);
             const bool there = FULL || at < n;
             ms[r] = there ? d.ms[t][at / ADAMW_SCALE_BLOCK] : 0.0f;
             rs[r] = there ? d.rs[t][at / ADAMW_SCALE_BLOCK] : 0.0f;
+            m[r] = v[r] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};      // (what a block behind the last one counts for below)
         }
     }
 #pragma unroll
@@ -178,7 +218,6 @@ __device__ __forceinline__ void adamw_chunk(const AdamwDesc<BITS> &d, int t, lon
         const long long at = base + (long long)r * ADAMW_BLOCK * 4, i = at + lane * 4;
         const int left = FULL ? 4 : n - i >= 4 ? 4 : n - i > 0 ? (int)(n - i) : 0;
         if (!FULL && at >= n) break;            // (uniform over the wave)
-        f32x4 root;
         if constexpr (BITS == 8) {
             m[r] = AdamwCodes::decode(cm[r], ms[r]);
             v[r] = AdamwCodes::decode(cr[r], rs[r]);
@@ -186,25 +225,40 @@ __device__ __forceinline__ void adamw_chunk(const AdamwDesc<BITS> &d, int t, lon
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float mj = m[r][j], vj = v[r][j], rj;
-            p[r][j] = adamw_update(d.k, p[r][j], g[r][j], mj, vj, rj);
-            m[r][j] = mj; v[r][j] = vj; root[j] = rj;
+            float mj = m[r][j], vj = v[r][j], root;
+            p[r][j] = adamw_update(d.k, p[r][j], g[r][j], mj, vj, root);
+            m[r][j] = mj;
+            v[r][j] = BITS == 8 ? root : vj;
         }
-        AdamwQuad<T>::store(d.p[t], i, left, p[r]);
+        AdamwQuad<T>::template store<false>(d.p[t], i, left, p[r]);
         if constexpr (BITS == 32) {
-            AdamwQuad<float>::store(d.m[t], i, left, m[r]);
-            AdamwQuad<float>::store(d.v[t], i, left, v[r]);
-        } else {
+            AdamwQuad<float>::store<STREAM>(d.m[t], i, left, m[r]);
+            AdamwQuad<float>::store<STREAM>(d.v[t], i, left, v[r]);
+        }
+    }
+    if constexpr (BITS == 8) {
+        unsigned top[2 * ADAMW_ROUNDS];
+#pragma unroll
+        for (int r = 0; r < ADAMW_ROUNDS; ++r) {
+            top[2 * r] = AdamwCodes::most(m[r]);
+            top[2 * r + 1] = AdamwCodes::most(v[r]);
+        }
+        wave_max_all(top);
+#pragma unroll
+        for (int r = 0; r < ADAMW_ROUNDS; ++r) {
+            const long long at = base + (long long)r * ADAMW_BLOCK * 4, i = at + lane * 4;
+            const int left = FULL ? 4 : n - i >= 4 ? 4 : n - i > 0 ? (int)(n - i) : 0;
+            if (!FULL && at >= n) break;
             float sm, sr;
-            const unsigned nm = AdamwCodes::encode<false>(m[r], sm), nr = AdamwCodes::encode<true>(root, sr);
-            AdamwCodes::store(d.m[t], i, left, nm);
-            AdamwCodes::store(d.r[t], i, left, nr);
+            const unsigned nm = AdamwCodes::encode<false>(m[r], top[2 * r], sm), nr = AdamwCodes::encode<true>(v[r], top[2 * r + 1], sr);
+            AdamwCodes::store<STREAM>(d.m[t], i, left, nm);
+            AdamwCodes::store<STREAM>(d.r[t], i, left, nr);
             if (lane == 0) { d.ms[t][at / ADAMW_SCALE_BLOCK] = sm; d.rs[t][at / ADAMW_SCALE_BLOCK] = sr; }
         }
     }
 }
 
-template <typename T, int BITS>
+template <typename T, int BITS, bool STREAM>
 __global__ __launch_bounds__(ADAMW_BLOCK) void adamw_kernel(const AdamwDesc<BITS> d)
 {
     // the tensor of this chunk: the number of running totals that are not above it (64 lanes look at two each)
@@ -214,6 +268,6 @@ __global__ __launch_bounds__(ADAMW_BLOCK) void adamw_kernel(const AdamwDesc<BITS
     const unsigned first = t ? d.end_chunk[t - 1] : 0u;
     const long long n = d.n[t], chunk = (long long)(blockIdx.x - first) * ADAMW_CHUNK;
     const long long base = chunk + (threadIdx.x >> 6) * ADAMW_SCALE_BLOCK;
-    if (chunk + ADAMW_CHUNK <= n) adamw_chunk<T, BITS, true>(d, t, n, base);
-    else adamw_chunk<T, BITS, false>(d, t, n, base);
+    if (chunk + ADAMW_CHUNK <= n) adamw_chunk<T, BITS, true, STREAM>(d, t, n, base);
+    else adamw_chunk<T, BITS, false, STREAM>(d, t, n, base);
 }

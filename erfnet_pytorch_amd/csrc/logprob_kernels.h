@@ -456,7 +456,8 @@ __device__ __forceinline__ float lp_grad(float x, float m, float log_s, float G,
 
 // GROUP threads take a segment of a row (GROUP = 64: the whole row).  The backward kernels walk from the last row to the
 // first: what forward read last is what the 256 MB cache still has (6 x 20 x 512 x 1024 fp32: 129 -> 125 us).
-template <typename T, int GROUP>
+// STREAM: the gradient is written past the caches (LP_STREAM in train_ops.hip).
+template <typename T, int GROUP, bool STREAM>
 __global__ __launch_bounds__(LP_BLOCK) void lp_rows_bwd_kernel(const LpDesc d)
 {
     constexpr int N = Vec16<T>::N;
@@ -496,7 +497,7 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_rows_bwd_kernel(const LpDesc d)
             Vec16<T>::unpack(ld16(x + c, to - c), v);
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] = none ? 0.0f : lp_grad(v[i], st.x, st.y, G, gh, H);
-            st16(dx + c, v, to - c);
+            st16<STREAM>(dx + c, v, to - c);
         }
     }
     // the gathered entries of this segment again, with what was gathered: after the block's plain stores
@@ -642,7 +643,7 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_pixels_kernel(const LpDesc d)
     }
 }
 
-template <typename T, int K>
+template <typename T, int K, bool STREAM>
 __global__ __launch_bounds__(LP_BLOCK) void lp_pixels_bwd_kernel(const LpDesc d)
 {
     const long long p = (long long)(gridDim.x - 1 - blockIdx.x) * LP_BLOCK + threadIdx.x;
@@ -668,10 +669,14 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_pixels_bwd_kernel(const LpDesc d)
     }
 #pragma unroll 4
     for (int c = 0; c < d.V; ++c) {
-        float g = lp_grad(Vec16<T>::get(x + c * d.next), st.x, st.y, G, gh, H);
+        const T xi = STREAM ? __builtin_nontemporal_load(x + c * d.next) : x[c * d.next];
+        float g = lp_grad(Vec16<T>::get(&xi), st.x, st.y, G, gh, H);
         if (c == (int)t) g += glp;
 #pragma unroll
         for (int j = 0; j < K; ++j) g += idx[j] == c ? gt[j] : 0.0f;
-        Vec16<T>::put(dx + (long long)c * d.inner, none ? 0.0f : g);
+        T gi;
+        Vec16<T>::put(&gi, none ? 0.0f : g);
+        if (STREAM) __builtin_nontemporal_store(gi, dx + (long long)c * d.inner);
+        else dx[(long long)c * d.inner] = gi;
     }
 }

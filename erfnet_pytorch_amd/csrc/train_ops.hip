@@ -174,6 +174,18 @@ bool lp_by_thread(long long outer, int V, long long inner, int k)
 #define LP_WAVE_BACKWARD 1024
 #define LP_BACKWARD_SEGMENT 8192
 
+// Backward: a gradient of 48 MB or more is written past the caches, so that the logits stay in the 256 MB one until they are
+// read again (pixels: that reading is their last, and goes past them too).  Forward and backward / the same with a reader of
+// the gradient behind them, us, ordinary and streamed: rows of 100003 bf16, 30 MB 24.7 / 35.2 and 25.0 / 38.9, 61 MB 43.1 / 64.0
+// and 41.2 / 64.2, 195 MB 123 / 187 and 109 / 179, 390 MB 236 / 363 and 212 / 356; 20 classes of fp32 pixels, 40 MB 29.6 / 43.2
+// and 30.0 / 44.3, 60 MB 45.8 / 67.6 and 43.2 / 63.8, 240 MB 185 / 267 and 178 / 258.
+#define LP_STREAM (48ll << 20)
+template <typename F> void lp_streamed(bool stream, F launch)
+{
+    if (stream) launch(std::true_type());
+    else launch(std::false_type());
+}
+
 // Forward, blocks per row: longer rows take whole blocks of at least 4096 classes, several to a row until there are 8192 of
 // them (2048 are resident; more rounds even out what the memory channels give each block), or 4096 where every block also finds
 // alternatives and a row's blocks have theirs to join.  Behind a 512 MB write that empties the caches, 2047 x 100003 bf16,
@@ -278,30 +290,43 @@ int lp_backward(const void *x, const long long *target, const float *entropy, co
     d.x = x; d.target = target; d.entropy = const_cast<float *>(entropy); d.stats = (float2 *)const_cast<float *>(stats);
     d.top_idx = const_cast<long long *>(top_idx); d.g_lp = g_lp; d.g_h = g_h; d.g_top = g_top; d.dx = dx;
     d.rows = outer * inner; d.ld = ld; d.inner = inner; d.ignore = ignore; d.V = V; d.k = k;
+    const bool stream = d.rows * V * (long long)sizeof(T) >= LP_STREAM;
     if (inner > 1) {
         d.group = V * inner;
         d.next = inner;
         const unsigned blocks = (unsigned)((d.rows + LP_BLOCK - 1) / LP_BLOCK);
-        if (!g_top || k == 0) lp_pixels_bwd_kernel<T, 0><<<blocks, LP_BLOCK, 0, st>>>(d);
-        else if (k <= 2) lp_pixels_bwd_kernel<T, 2><<<blocks, LP_BLOCK, 0, st>>>(d);
-        else lp_pixels_bwd_kernel<T, 8><<<blocks, LP_BLOCK, 0, st>>>(d);
+        lp_streamed(stream, [&](auto stream) {
+            if (!g_top || k == 0) lp_pixels_bwd_kernel<T, 0, stream><<<blocks, LP_BLOCK, 0, st>>>(d);
+            else if (k <= 2) lp_pixels_bwd_kernel<T, 2, stream><<<blocks, LP_BLOCK, 0, st>>>(d);
+            else lp_pixels_bwd_kernel<T, 8, stream><<<blocks, LP_BLOCK, 0, st>>>(d);
+        });
         LAUNCHED("lp_pixels_bwd_kernel");
         return 0;
     }
     if (V <= LP_SHORT && outer >= LP_SHORT_BACKWARD * V) {
         lp_short_rows_bwd_kernel<T><<<(unsigned)((outer + LP_SHORT_ROWS - 1) / LP_SHORT_ROWS), LP_BLOCK, 0, st>>>(d);
     } else if (V <= LP_WAVE_BACKWARD) {
-        lp_rows_bwd_kernel<T, 64><<<(unsigned)((outer + 3) / 4), LP_BLOCK, 0, st>>>(d);
+        lp_streamed(stream, [&](auto stream) {
+            lp_rows_bwd_kernel<T, 64, stream><<<(unsigned)((outer + 3) / 4), LP_BLOCK, 0, st>>>(d);
+        });
     } else {
         d.seg = LP_BACKWARD_SEGMENT;
         d.splits = (V + d.seg - 1) / d.seg;
-        lp_rows_bwd_kernel<T, 256><<<(unsigned)(outer * d.splits), LP_BLOCK, 0, st>>>(d);
+        lp_streamed(stream, [&](auto stream) {
+            lp_rows_bwd_kernel<T, 256, stream><<<(unsigned)(outer * d.splits), LP_BLOCK, 0, st>>>(d);
+        });
     }
     LAUNCHED("lp_rows_bwd_kernel");
     return 0;
 }
 
 // ================================================================================ AdamW
+// Tensors (parameters, gradients, moments) of this many bytes in all are read past the caches, and their moments, which nobody
+// reads before the next step, are written past them.  Ordinary and streamed, us: bf16 with fp32 moments, 256 MB: steps one
+// behind the other 74 and 80, behind a 400 MB write and with a reader of the parameters 117 and 102; 320 MB 101 / 141 and 99 /
+// 128; 400 MB 146 / 174 and 121 / 161; 720 MB 258 / 309 and 213 / 284.  fp32 with 8-bit ones, 320 MB 97 / 156 and 96 / 149, 720 MB 232 /
+// 345 and 208 / 343.
+#define ADAMW_STREAM (320ll << 20)
 template <typename T, int BITS>
 int adamw_step(const char *what, int count, void *const *p, const void *const *g, void *const *m, float *const *ms,
                void *const *v, float *const *vs, const long long *numel, double lr, double b1, double b2, double eps,
@@ -318,10 +343,12 @@ int adamw_step(const char *what, int count, void *const *p, const void *const *g
     d.k.b1 = (float)b1; d.k.ob1 = (float)(1.0 - b1); d.k.b2 = (float)b2; d.k.ob2 = (float)(1.0 - b2);
     d.k.keep = (float)(1.0 - lr * wd);
     d.k.step = (float)(lr / (1.0 - pow(b1, (double)step)));
-    d.k.root_c2 = (float)sqrt(1.0 - pow(b2, (double)step));
+    d.k.inv_root_c2 = (float)(1.0 / sqrt(1.0 - pow(b2, (double)step)));
     d.k.eps = (float)eps;
+    long long elements = 0;
     for (int i = 0; i < count; ++i) {
         if (numel[i] < 0) return fail("%s: tensor %d has a negative size", what, i);
+        elements += numel[i];
         if (numel[i] && (!p[i] || !g[i] || !m[i] || !v[i] || (BITS == 8 && (!ms[i] || !vs[i]))))
             return fail("%s: tensor %d has a null pointer", what, i);
         if (numel[i] / ADAMW_CHUNK >= (1ll << 31) - 1) return fail("%s: tensor %d is too large", what, i);
@@ -333,6 +360,7 @@ int adamw_step(const char *what, int count, void *const *p, const void *const *g
         (void)hipGetLastError();
         return fail("%s: the step cannot be captured into a graph", what);
     }
+    const bool stream = elements >= ADAMW_STREAM / (2 * (long long)sizeof(T) + (BITS == 8 ? 2 : 8));
     int i = 0;
     while (i < count) {
         d.count = 0;
@@ -350,7 +378,8 @@ int adamw_step(const char *what, int count, void *const *p, const void *const *g
             d.end_chunk[k] = (unsigned)chunks;
         }
         if (d.count == 0) continue;
-        adamw_kernel<T, BITS><<<(unsigned)chunks, ADAMW_BLOCK, 0, st>>>(d);
+        if (stream) adamw_kernel<T, BITS, true><<<(unsigned)chunks, ADAMW_BLOCK, 0, st>>>(d);
+        else adamw_kernel<T, BITS, false><<<(unsigned)chunks, ADAMW_BLOCK, 0, st>>>(d);
         LAUNCHED("adamw_kernel");
     }
     return 0;

@@ -80,13 +80,23 @@ template <typename T> __device__ __forceinline__ u32x4 ld16(const T *p, int left
     }
     return r;
 }
+// An access that leaves the caches to others (STREAM), or an ordinary one; V is a packed struct around a vector.
+template <bool STREAM, typename V> __device__ __forceinline__ auto ld_vec(const V *p)
+{
+    return STREAM ? __builtin_nontemporal_load(&p->v) : p->v;
+}
+template <bool STREAM, typename V, typename R> __device__ __forceinline__ void st_vec(V *p, R r)
+{
+    if (STREAM) __builtin_nontemporal_store(r, &p->v);
+    else p->v = r;
+}
 // The first `left` elements of f: 16 bytes, or the partial vector in pieces of 8, 4 and 2.
-template <typename T> __device__ __forceinline__ void st16(T *p, const float (&f)[Vec16<T>::N], int left)
+template <bool STREAM = false, typename T> __device__ __forceinline__ void st16(T *p, const float (&f)[Vec16<T>::N], int left)
 {
     typedef typename Vec16<T>::Raw Raw;
     u32x4 r = Vec16<T>::pack(f);
     if (left >= Vec16<T>::N) {
-        reinterpret_cast<Raw *>(p)->v = r;
+        st_vec<STREAM>(reinterpret_cast<Raw *>(p), r);
         return;
     }
     if (left <= 0) return;

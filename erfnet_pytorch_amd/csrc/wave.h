@@ -72,3 +72,35 @@ __device__ __forceinline__ float wave_max(float v, int lanes = 64)
 {
     return wave_reduce(v, lanes, [](float a, float b) { return fmaxf(a, b); });
 }
+// Maxima of N values (4 or 8) over the whole wave, as scalars.  The first two steps each join two registers into one that holds
+// a half (a row of 16) of either, so that N / 4 registers take the last four: 7 steps for 4 values instead of 24.
+template <int N> __device__ __forceinline__ void wave_max_all(unsigned (&v)[N])
+{
+    unsigned a[N / 2], b[N / 4];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {           // lanes below 32: v[2 i], the others v[2 i + 1]
+        const auto r = __builtin_amdgcn_permlane32_swap(v[2 * i], v[2 * i + 1], false, false);
+        const unsigned x = r[0], y = r[1];
+        a[i] = x > y ? x : y;
+    }
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {           // rows: v[4 i], v[4 i + 2], v[4 i + 1], v[4 i + 3]
+        const auto r = __builtin_amdgcn_permlane16_swap(a[2 * i], a[2 * i + 1], false, false);
+        const unsigned x = r[0], y = r[1];
+        b[i] = x > y ? x : y;
+    }
+    auto step = [](unsigned x, int y) { return x > (unsigned)y ? x : (unsigned)y; };
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) b[i] = step(b[i], __builtin_amdgcn_update_dpp((int)b[i], (int)b[i], 0xb1, 0xf, 0xf, false));
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) b[i] = step(b[i], __builtin_amdgcn_update_dpp((int)b[i], (int)b[i], 0x4e, 0xf, 0xf, false));
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) b[i] = step(b[i], __builtin_amdgcn_update_dpp((int)b[i], (int)b[i], 0x141, 0xf, 0xf, false));
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) b[i] = step(b[i], __builtin_amdgcn_update_dpp((int)b[i], (int)b[i], 0x140, 0xf, 0xf, false));
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            v[4 * i + j] = (unsigned)__builtin_amdgcn_readlane((int)b[i], 16 * ((j & 1) * 2 + (j >> 1)));
+}
