@@ -79,7 +79,7 @@ def build(force=False, verbose=False):
         lib_dir = os.path.join(base, "lib")
         _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", *("-I" + i for i in inc),
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__", _HOST_SRC, "-o", _HOST_SO, "-L" + lib_dir,
-              "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath," + lib_dir], verbose)
+              "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-Wl,-rpath," + lib_dir], verbose)
     srcs = sources()
     if not force and os.path.exists(_SO) and \
             os.path.getmtime(_SO) >= max(os.path.getmtime(s) for s in srcs):

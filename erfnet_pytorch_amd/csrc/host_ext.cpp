@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -49,6 +50,12 @@ void check(int rc)
 }
 void *stream(const c10::Device &d) { return c10::hip::getCurrentHIPStream(d.index()).stream(); }
 float *floats(const Tensor &t) { return t.defined() ? (float *)t.data_ptr() : nullptr; }
+// (not through the dispatcher, which takes as long as the allocation: there are up to seven of these in a call)
+Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const Tensor &beside, bool image = false)
+{
+    return Tensor(at::detail::empty_cuda(shape, type, beside.device(),
+                                         image ? at::MemoryFormat::ChannelsLast : at::MemoryFormat::Contiguous));
+}
 Tensor parameter(const Tensor &t) { return t.defined() ? t.to(at::kFloat).contiguous() : t; }
 
 // What backward returns, from an operator whose gradient has none: where a graph of the backward pass is recorded
@@ -80,8 +87,8 @@ Tensor norm_forward(const Tensor &x, const Tensor &w, const Tensor &b, double ep
     const int64_t c = x.size(image ? 1 : -1), rows = x.numel() / c;
     const c10::DeviceGuard guard(x.device());
     const Tensor wf = parameter(w), bf = parameter(b);
-    Tensor y = at::empty_like(x);
-    if (stat) *stat = at::empty({2, rows}, x.options().dtype(at::kFloat));
+    Tensor y = fresh(x.sizes(), x.scalar_type(), x, image);
+    if (stat) *stat = fresh({2, rows}, at::kFloat, x);
     float *kept = stat ? floats(*stat) : nullptr;
     check(lib.norm_fwd[kind(x)](x.data_ptr(), floats(wf), floats(bf), y.data_ptr(), kept, kept ? kept + rows : nullptr, rows,
                                 (int)c, (float)eps, stream(x.device())));
@@ -112,15 +119,14 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const at::AutoGradMode off(false);
         const Tensor gy = norm_rows(grads[0].to(x.scalar_type()), image), wf = parameter(w);
         Tensor dx, dw, db, ws;
-        if (ctx->needs_input_grad(0)) dx = at::empty_like(x);
-        const auto f32 = x.options().dtype(at::kFloat);
+        if (ctx->needs_input_grad(0)) dx = fresh(x.sizes(), x.scalar_type(), x, image);
         // (an absent weight has no edge)
-        if (w.defined() && ctx->needs_input_grad(1)) dw = at::empty({c}, f32);
-        if (bias >= 0 && ctx->needs_input_grad(w.defined() ? 2 : 1)) db = at::empty({c}, f32);
+        if (w.defined() && ctx->needs_input_grad(1)) dw = fresh({c}, at::kFloat, x);
+        if (bias >= 0 && ctx->needs_input_grad(w.defined() ? 2 : 1)) db = fresh({c}, at::kFloat, x);
         int64_t n_ws = 0;
         if (dw.defined() || db.defined()) {
             n_ws = (int64_t)lib.norm_ws(rows, (int)c);
-            ws = at::empty({n_ws}, x.options().dtype(at::kByte));
+            ws = fresh({n_ws}, at::kByte, x);
         }
         check(lib.norm_bwd[kind(x)](x.data_ptr(), floats(wf), floats(stat), floats(stat) + rows, gy.data_ptr(),
                                     dx.defined() ? dx.data_ptr() : nullptr, floats(dw), floats(db), rows, (int)c,
@@ -170,13 +176,11 @@ variable_list logp_forward(const Tensor &logits, const Tensor &target0, LogpShap
         if (i != s.axis) full.push_back(logits.size(i));
         else if (!s.moved) full.push_back(s.top_k);
     if (s.moved) full.push_back(s.top_k);
-    const auto f32 = logits.options().dtype(at::kFloat);
-    const Tensor lp = at::empty(target.sizes(), f32), ent = at::empty(target.sizes(), f32), top = at::empty(full, f32);
-    const Tensor idx = at::empty(full, f32.dtype(at::kLong));
-    const Tensor stats = at::empty({2 * pixels}, f32);
+    const Tensor lp = fresh(target.sizes(), at::kFloat, x), ent = fresh(target.sizes(), at::kFloat, x);
+    const Tensor top = fresh(full, at::kFloat, x), idx = fresh(full, at::kLong, x), stats = fresh({2 * pixels}, at::kFloat, x);
     Tensor ws;
     const int64_t n_ws = (int64_t)lib.logp_ws(s.outer, (int)s.v, s.inner, (int)s.top_k);
-    if (n_ws) ws = at::empty({n_ws}, f32.dtype(at::kByte));
+    if (n_ws) ws = fresh({n_ws}, at::kByte, x);
     check(lib.logp_fwd[kind(x)](x.data_ptr(), (const long long *)target.data_ptr(), floats(lp), floats(ent), floats(stats), floats(top),
                                 (long long *)idx.data_ptr(), s.outer, (int)s.v, s.inner, s.ld, (int)s.top_k, s.ignore,
                                 ws.defined() ? ws.data_ptr() : nullptr, (size_t)n_ws, stream(x.device())));
@@ -217,7 +221,7 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
             shape.push_back(shape[axis]);
             shape.erase(shape.begin() + axis);
         }
-        Tensor dx = at::empty(shape, x.options());
+        Tensor dx = fresh(shape, x.scalar_type(), x);
         check(lib.logp_bwd[kind(x)](x.data_ptr(), (const long long *)target.data_ptr(), floats(ent), floats(stats),
                                     (const long long *)idx.data_ptr(), floats(g[0]), floats(g[1]), floats(g[2]), dx.data_ptr(),
                                     s[0], (int)s[1], s[2], s[3], (int)s[4], s[5], stream(x.device())));
