@@ -192,13 +192,28 @@ struct LpTurns {
     __device__ __forceinline__ int begin(int quarter) const { return turns * quarter / 4; }
 };
 
-// What one thread does with its share of elements [from, to) of a row: 16 at a time in vectors `threads` apart, with the
-// next ones' loads in flight; the last turn, which may lack some, by itself.  TOP: high[0..3] receive the quarters' maxima.
+// Elements in front of the first cache line that begins at or behind p.
+template <typename T> __device__ __forceinline__ int lp_head(const T *p, int left)
+{
+    const int h = (int)(-(unsigned)(unsigned long long)p & 127u) / (int)sizeof(T);
+    return h < left ? h : left;
+}
+
+// What one thread does with its share of elements [from, to) of a row: one of the `first` that precede a cache line's
+// beginning, then 16 at a time in vectors `threads` apart, with the next ones' loads in flight; the last turn, which may lack
+// some, by itself.  TOP: high[0..3] receive the quarters' maxima (without the head's, which is given back).
 template <typename T, bool TOP>
-__device__ __forceinline__ LpSums lp_scan(const T *x, int from, int to, int me, int threads, float (&high)[4])
+__device__ __forceinline__ LpSums lp_scan(const T *x, int from, int first, int to, int me, int threads, float &head, float (&high)[4])
 {
     constexpr int N = Vec16<T>::N, U = 16 / N;
     LpSums r = {LP_LOWEST, 0.0f, 0.0f};
+    head = -INFINITY;
+    if (me < first) {
+        head = Vec16<T>::get(x + from + me);
+        if (head > r.m) lp_move(r, head);
+        lp_add(r, head);
+    }
+    from += first;
     const LpTurns plan(from, to, threads, N, U);
     const int step = plan.step, turns = plan.turns;
     const T *at = x + from + me * N;
@@ -355,15 +370,19 @@ __global__ __launch_bounds__(LP_BLOCK, 8) void lp_rows_kernel(const LpDesc d)
         to = from + d.seg < d.V ? from + d.seg : d.V;
     }
     const T *x = (const T *)d.x + row * d.ld;
-    float quarters[4];
-    LpSums r = lp_scan<T, TOP>(x, from, to, me, GROUP, quarters);
+    float head, quarters[4];
+    // Blocks stream long rows and begin at a cache line: their waves would share one at either end of every vector, and with 32 of
+    // them on a compute unit it is fetched twice (4096 x 130001 bf16, top 8: 248 -> 209 us).  A wave that has a short row to
+    // itself is faster without the detour (8192 x 3001: 20 and 23).
+    const int first = GROUP == 256 ? lp_head(x + from, to - from) : 0;
+    LpSums r = lp_scan<T, TOP>(x, from, first, to, me, GROUP, head, quarters);
     LpList top;
     if (TOP) {
         top.buf = (lp_lds64 *)buf[wave];
         // a thread's largest key, or a bound below it: the sums are NaN where it holds a NaN (which the maximum does not
         // show) or +infinity; 0 where it holds nothing
         const bool spoilt = r.s != r.s;
-        const unsigned mine = from + me * Vec16<T>::N >= to ? 0u : spoilt ? lp_key32(INFINITY)
+        const unsigned mine = me >= first && from + first + me * Vec16<T>::N >= to ? 0u : spoilt ? lp_key32(INFINITY)
                               : r.s == 0.0f ? lp_key32(-INFINITY) : lp_key32(r.m);
         unsigned best = lp_sort64(mine);
         if (GROUP == 256) {
@@ -371,8 +390,10 @@ __global__ __launch_bounds__(LP_BLOCK, 8) void lp_rows_kernel(const LpDesc d)
             __syncthreads();
             for (int w = 1; w < 4; ++w) best = lp_merge(best, high[(wave + w) & 3][lane]);
         }
-        const unsigned bar = (unsigned)__builtin_amdgcn_readlane((int)best, d.k - 1);
-        lp_collect<T>(x, from, to, GROUP == 256 ? wave * 64 : 0, GROUP, quarters, spoilt, bar > 1u ? bar : 1u, d.k,
+        unsigned bar = (unsigned)__builtin_amdgcn_readlane((int)best, d.k - 1);
+        if (bar < 1u) bar = 1u;
+        if (GROUP == 256) top.offer(me < first && lp_key32(head) >= bar ? lp_key(head, from + me) : 0ull, d.k);
+        lp_collect<T>(x, from + first, to, GROUP == 256 ? wave * 64 : 0, GROUP, quarters, spoilt, bar, d.k,
                       (lp_lds8 *)owners[wave], top);
     }
     r = lp_wave_join(r);

@@ -168,9 +168,12 @@ bool lp_by_thread(long long outer, int V, long long inner, int k)
 {
     return inner > 1 || (V <= LP_SHORT && k <= ERF_LOG_PROBS_MAX_TOP_PIXELS && outer >= LP_SHORT_FORWARD * V);
 }
-// Forward: a wave takes a row of up to 4096 classes (8192 x 4000 bf16, top 8: 23 us, 42 with a block a row; 8192 x 8000 fp32: 65
-// and 55); backward, which has no results to join, of up to 1024 (8192 x 1000 bf16: 8.0 and 11.6 us, 8192 x 4000: 23.1 and 21.8).
-#define LP_WAVE_FORWARD 4096
+// Forward: a wave takes a row of up to 32 KB, 16 KB where its lists are long (they are merged once a row by a wave, by four
+// in a block), and of up to 4 KB where there are too few rows for the card; a block takes the others (us, a wave / a block
+// a row, top 8 and 32: 8192 x 4096 bf16 25 / 41 and 28 / 42, 8192 x 8192 39 / 50 and 45 / 51, 8192 x 16384 62 / 68 and 81 / 68, 4096 x 24001
+// 46 / 51 and 63 / 54; fp32 8192 x 8192 57 / 53 and 76 / 60; 512 x 6001 bf16 10.4 / 10.0 and 13.6 / 10.3).
+// Backward, which has no results to join: a wave of up to 1024 classes (8192 x 1000 bf16: 8.0 and 11.6 us, 8192 x 4000: 23.1 and
+// 21.8).
 #define LP_WAVE_BACKWARD 1024
 #define LP_BACKWARD_SEGMENT 8192
 
@@ -186,29 +189,30 @@ template <typename F> void lp_streamed(bool stream, F launch)
     else launch(std::false_type());
 }
 
-// Forward, blocks per row: longer rows take whole blocks of at least 4096 classes, several to a row until there are 8192 of
-// them (2048 are resident; more rounds even out what the memory channels give each block), or 4096 where every block also finds
-// alternatives and a row's blocks have theirs to join.  Behind a 512 MB write that empties the caches, 2047 x 100003 bf16,
-// 1 / 2 / 3 / 5 blocks a row: 146 / 150 / 138 / 131 us without alternatives, 155 / 158 / 149 / 149 with 8; 300 x 131072,
-// 3 / 7 / 14 / 32 a row, with 8: 44 / 47 / 45 / 59.
+// Forward: where there are few long rows, each takes several blocks of at least 4096 classes, until there are 512, and the
+// join's launch after them (us, top 8, one block / 512 in all: 8 x 100003 bf16 17.9 / 12.7, 64 x 131072 21 / 17, 256 x 131072 22 / 23, 8 x 50000 12.7 /
+// 12.1; more of them cost more than they bring: 1024 x 50003, 1 / 4 a row 28 / 45, 2047 x 100003 87 / 96).
+#define LP_FEW_ROWS 128
+#define LP_LONG_ROW 65536
 struct LpPlan {
     bool wave;
     int splits, seg;
 };
-LpPlan lp_plan(long long rows, int V, int k)
+template <typename T> LpPlan lp_plan(long long rows, int V, int k)
 {
-    LpPlan p = {V <= LP_WAVE_FORWARD, 1, V};
-    if (p.wave) return p;
-    const long long want = ((k ? 4096 : 8192) + rows - 1) / std::max<long long>(rows, 1);
-    p.splits = (int)std::min<long long>(std::max<long long>(want, 1), (V + 4095) / 4096);
+    const long long most = rows < 1024 ? 4096 : k > 16 ? 16384 : 32768;
+    LpPlan p = {V * (long long)sizeof(T) <= most, 1, V};
+    if (p.wave || rows > LP_FEW_ROWS || V < LP_LONG_ROW) return p;
+    p.splits = (int)std::min<long long>(512 / std::max<long long>(rows, 1), (V + 4095) / 4096);
     p.seg = ((V + p.splits - 1) / p.splits + 4095) / 4096 * 4096;
     p.splits = (V + p.seg - 1) / p.seg;
     return p;
 }
+// (the same for both types: rows that are split are longer than a wave takes)
 size_t lp_ws(long long outer, int V, long long inner, int k)
 {
     if (lp_by_thread(outer, V, inner, k)) return 0;
-    const LpPlan p = lp_plan(outer, V, k);
+    const LpPlan p = lp_plan<bf16_t>(outer, V, k);
     return p.splits > 1 ? (size_t)outer * p.splits * (sizeof(float4) + (size_t)k * 8) : 0;
 }
 
@@ -252,7 +256,7 @@ int lp_forward(const void *x, const long long *target, float *log_prob, float *e
         LAUNCHED("lp_pixels_kernel");
         return 0;
     }
-    const LpPlan p = lp_plan(outer, V, k);
+    const LpPlan p = lp_plan<T>(outer, V, k);
     d.splits = p.splits; d.seg = p.seg;
     if (p.splits > 1) {
         if (!ws || ws_bytes < lp_ws(outer, V, inner, k)) return fail("log_probs: workspace too small");
