@@ -67,16 +67,19 @@ template <typename T, typename F> void norm_by_shape(const NormPlan &p, int C, F
     if (C % Vec16<T>::N == 0) with(std::true_type());
     else with(std::false_type());
 }
-// Blocks that walk over the rows: as many as the card holds at once, `threads` of them on a compute unit.  Backward takes
-// at least `turns` rows a thread beyond one block per unit, so that the blocks' partial sums stay a small part of its traffic.
+// Blocks that walk over the rows, with `threads` threads on a compute unit in all.  Backward takes at least `turns` rows a
+// thread beyond one block per unit, so that the blocks' partial sums stay a small part of its traffic.
 int norm_blocks(const NormPlan &p, long long rows, int threads, int turns)
 {
     const long long per = p.wave ? NORM_BLOCK / p.lanes : 1;
     const long long all = (rows + per - 1) / per, full = 256ll * std::max(1, threads / p.threads);
     return (int)std::min(std::min(all, full), std::max<long long>(256, all / turns));
 }
-#define NORM_FWD_BLOCKS(p, rows) norm_blocks(p, rows, 2048, 1)
-#define NORM_BWD_BLOCKS(p, rows) norm_blocks(p, rows, 1024, 8)
+// (us: forward with 2048 / 1024 threads a unit, 8191 x 8192 bf16 47 / 43, 49152 x 128 fp32 9.3 / 9.6; backward, a wave a row, 1024
+// / 512, 20000 x 1000 fp32 54 / 50, 786432 x 16 bf16 20.6 / 19.2; a block a row, 1024 / 512 / 256, 8191 x 4096 bf16 67 / 51 / 47, 8191 x 8192 97 /
+// 86 / 86, 8191 x 2048 35 / 35 / 31)
+#define NORM_FWD_BLOCKS(p, rows) norm_blocks(p, rows, 1024, 1)
+#define NORM_BWD_BLOCKS(p, rows) norm_blocks(p, rows, (p).wave ? 512 : 256, 8)
 
 // (partial sums of wide rows, us with 16 / 64 columns a block: C = 2048 12.6 / 11.8, 4096 11.9 / 8.1, 8192 13.3 / 7.3; 16 below,
 // where 64 leave most compute units without a block)
