@@ -261,18 +261,47 @@ __device__ __forceinline__ LpSums lp_scan(const T *x, int from, int first, int t
     return r;
 }
 
+// A vector's entries that reach `bar`, into top, one from each lane a turn, the lowest first (left <= 0: none).
+template <typename T>
+__device__ __forceinline__ void lp_take(const T *x, int c, int left, unsigned bar, int k, LpList &top)
+{
+    constexpr int N = Vec16<T>::N;
+    float v[N];
+    Vec16<T>::unpack(ld16(x + c, left), v);
+    unsigned mine = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine |= (i < left) & (lp_key32(v[i]) >= bar) ? 1u << i : 0u;
+    while (__ballot(mine != 0u)) {
+        const int j = __ffs(mine) - 1;          // (-1: nothing left, the selection below gives any of them)
+        // element j by bit selection (written as ternaries it becomes an indexed register file)
+        unsigned f[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = __builtin_bit_cast(unsigned, v[i]);
+#pragma unroll
+        for (int half = N / 2; half > 0; half >>= 1) {
+            unsigned pick = (j & half) ? ~0u : 0u;
+            asm volatile("" : "+v"(pick));
+#pragma unroll
+            for (int i = 0; i < half; ++i) f[i] = (f[i] & ~pick) | (f[i + half] & pick);
+        }
+        top.offer(mine ? lp_key(__builtin_bit_cast(float, f[0]), c + j) : 0ull, k);
+        mine &= mine - 1u;
+    }
+}
+
+#define LP_MANY 512             // vectors
 // The entries of this wave's threads that reach `bar`, into top.  high: the threads' quarters' maxima; `spoilt`: they do not
-// show all there is.  A lane takes one vector of one quarter that reaches the bar at a time, so that the few there are
-// occupy the whole wave.  (Every such vector costs a cache line: by whole shares instead of quarters the second reading
-// fetched 28 % of a row of 100003 bf16 classes again, k = 8.)
+// show all there is; `best`: the largest key32 of any, if none is spoilt.  A lane takes one vector of one quarter that reaches
+// the bar at a time, so that the few there are occupy the whole wave.  (Every such vector costs a cache line: by whole shares
+// instead of quarters the second reading fetched 28 % of a row of 100003 bf16 classes again, k = 8.)
 template <typename T>
 __device__ __forceinline__ void lp_collect(const T *x, int from, int to, int first, int threads, const float (&high)[4],
-                                           bool spoilt, unsigned bar, int k, lp_lds8 *owners, LpList &top)
+                                           bool spoilt, unsigned bar, unsigned best, int k, lp_lds8 *owners, LpList &top)
 {
     constexpr int N = Vec16<T>::N, U = 16 / N;
     const LpTurns plan(from, to, threads, N, U);
     const int lane = threadIdx.x & 63, step = plan.step;
-    int n = 0;
+    int n = 0, upto[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const bool some = plan.begin(j) < plan.begin(j + 1) || (j == 3 && plan.left > 0);
@@ -281,34 +310,33 @@ __device__ __forceinline__ void lp_collect(const T *x, int from, int to, int fir
         const int at = n + __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
         if (owner) owners[at] = (unsigned char)(lane | j << 6);
         n += __popcll(mask);
+        upto[j] = n;
     }
     const int most = (plan.turns + 3) / 4 * U + (plan.left > 0 ? U : 0);       // vectors of a quarter, at most
-    for (int q0 = 0; q0 < n * most; q0 += 64) {     // (the same number of turns for all lanes: the votes need them)
-        const int q = q0 + lane, o = q / most, t = q - o * most;
-        const unsigned own = q < n * most ? owners[o] : 0u;
-        const int j = own >> 6, begin = plan.begin(j) * U, end = j == 3 ? begin + most : plan.begin(j + 1) * U;
-        const int c = from + (begin + t) * step + (first + (int)(own & 63u)) * N;
-        const int left = q < n * most && begin + t < end && c < to ? to - c : 0;
-        float v[N];
-        Vec16<T>::unpack(ld16(x + c, left), v);
-        unsigned mine = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) mine |= (i < left) & (lp_key32(v[i]) >= bar) ? 1u << i : 0u;
-        while (__ballot(mine != 0u)) {          // one entry from each lane a turn, the lowest first
-            const int j = __ffs(mine) - 1;      // (-1: nothing left, the selection below gives any of them)
-            // element j by bit selection (written as ternaries it becomes an indexed register file)
-            unsigned f[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) f[i] = __builtin_bit_cast(unsigned, v[i]);
-#pragma unroll
-            for (int half = N / 2; half > 0; half >>= 1) {
-                unsigned pick = (j & half) ? ~0u : 0u;
-                asm volatile("" : "+v"(pick));
-#pragma unroll
-                for (int i = 0; i < half; ++i) f[i] = (f[i] & ~pick) | (f[i + half] & pick);
-            }
-            top.offer(mine ? lp_key(__builtin_bit_cast(float, f[0]), c + j) : 0ull, k);
-            mine &= mine - 1u;
+    if (n * most <= LP_MANY) {
+        for (int q0 = 0; q0 < n * most; q0 += 64) {     // (the same number of turns for all lanes: the votes need them)
+            const int q = q0 + lane, o = q / most, t = q - o * most;
+            const unsigned own = q < n * most ? owners[o] : 0u;
+            const int j = own >> 6, begin = plan.begin(j) * U, end = j == 3 ? begin + most : plan.begin(j + 1) * U;
+            const int c = from + (begin + t) * step + (first + (int)(own & 63u)) * N;
+            lp_take(x, c, q < n * most && begin + t < end && c < to ? to - c : 0, bar, k, top);
+        }
+        return;
+    }
+    // Very many: in the order of the row, until the list is full of entries that nothing behind them can pass.  (All of a row of
+    // equal entries reach the bar, and a row of masked ones is such a row: with one in 61 of 2047 x 100003 bf16, k = 8, the others
+    // waited for them, 184 us; 92 so.  In this order always: 64 x 50000, k = 32, 17 us, 14 in the other.)
+    for (int j = 0; j < 4; ++j) {
+        const int o0 = j ? upto[j - 1] : 0, count = upto[j] - o0, begin = plan.begin(j) * U;
+        const int vectors = plan.begin(j + 1) * U - begin + (j == 3 && plan.left > 0 ? U : 0);
+        for (int q0 = 0; q0 < count * vectors; q0 += 64) {
+            const int lowest = from + (begin + q0 / count) * step + first * N;
+            if (best < lp_key32(INFINITY) && ((unsigned long long)best << 32 | (unsigned)~lowest) < top.kth) return;
+            const int q = q0 + lane, t = q / count;
+            const bool live = q < count * vectors;
+            const unsigned own = live ? owners[o0 + q - t * count] : 0u;
+            const int c = from + (begin + t) * step + (first + (int)(own & 63u)) * N;
+            lp_take(x, c, live && c < to ? to - c : 0, bar, k, top);
         }
     }
 }
@@ -393,8 +421,8 @@ __global__ __launch_bounds__(LP_BLOCK, 8) void lp_rows_kernel(const LpDesc d)
         unsigned bar = (unsigned)__builtin_amdgcn_readlane((int)best, d.k - 1);
         if (bar < 1u) bar = 1u;
         if (GROUP == 256) top.offer(me < first && lp_key32(head) >= bar ? lp_key(head, from + me) : 0ull, d.k);
-        lp_collect<T>(x, from + first, to, GROUP == 256 ? wave * 64 : 0, GROUP, quarters, spoilt, bar, d.k,
-                      (lp_lds8 *)owners[wave], top);
+        lp_collect<T>(x, from + first, to, GROUP == 256 ? wave * 64 : 0, GROUP, quarters, spoilt, bar,
+                      (unsigned)__builtin_amdgcn_readlane((int)best, 0), d.k, (lp_lds8 *)owners[wave], top);
     }
     r = lp_wave_join(r);
     if (GROUP == 64) {

@@ -442,6 +442,28 @@ def test_log_probs_alternatives_of_ordered_rows(v, how):
 
 
 @gpu
+@pytest.mark.parametrize("k", [1, 7, 64])
+@pytest.mark.parametrize("v,rows", [(9001, 5), (9001, 1100), (50003, 3), (100003, 2)])
+def test_log_probs_alternatives_among_many_ties(v, rows, k):
+    """Few distinct values (the lowest indices of the largest win, wherever it begins), masked rows and columns, rows at every
+    alignment: a wave a row, a block a row and several blocks a row."""
+    from erfnet_pytorch_amd import functional as hipf
+    g = torch.Generator().manual_seed(v + k)
+    x = torch.randint(0, 3, (5, v), generator=g).float()
+    x[1] = -float("inf")
+    x[2, : v // 2] = 0.0
+    x[3].clamp_(max=1.0)
+    x[3, -5:] = 2.0
+    x[4, torch.rand(v, generator=g) < 0.5] = -float("inf")
+    x = x.repeat(-(-rows // 5), 1)[:rows].contiguous()
+    t = torch.randint(0, v, (rows,), generator=g)
+    r = hipf.log_probs(x.to(DEV).bfloat16(), t.to(DEV), k)
+    ref = lp_reference(x[:5], t[:5], k, -1)
+    check_lp(hipf.LogProbs(*(o[:5] for o in r)), ref, (v, rows, k))
+    assert torch.equal(r.top_indices[-5:], r.top_indices[:5])       # (rows is below 5 or a multiple of it)
+
+
+@gpu
 def test_log_probs_last_position_of_padded_batch_and_leading_shapes():
     """logits[:, -1] of a [B, S, V] tensor is read in place with a row stride; a 1-D row; expanded rows; no rows."""
     from erfnet_pytorch_amd import functional as hipf
