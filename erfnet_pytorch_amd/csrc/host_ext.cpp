@@ -316,6 +316,26 @@ bool usable(const at::Tensor &t, const char *what)
     return true;
 }
 
+// A dict read in its own order, which is the order of the questions as a rule, and looked up where it is not.
+struct Walk {
+    PyObject *dict, *key = nullptr, *value = nullptr;
+    Py_ssize_t pos = 0;
+    bool more;
+    explicit Walk(PyObject *d) : dict(d) { more = PyDict_Next(dict, &pos, &key, &value); }
+    PyObject *next_if(PyObject *k)
+    {
+        if (!more || key != k) return nullptr;
+        PyObject *v = value;
+        more = PyDict_Next(dict, &pos, &key, &value);
+        return v;
+    }
+    PyObject *find(PyObject *k)             // (null without an error: not there)
+    {
+        PyObject *v = next_if(k);
+        return v ? v : PyDict_GetItemWithError(dict, k);
+    }
+};
+
 // adamw_step(params, state, keys, bits, lr, beta1, beta2, eps, weight_decay)
 //   params: list of Parameters; state: the optimiser's {Parameter: {key: tensor}}; keys: moments in the order of the
 //   library's tables.
@@ -342,21 +362,14 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     THPObjectPtr missing(PyList_New(0));
     if (!missing) return nullptr;
     std::vector<Batch> batches;
-    // the state dict holds the parameters in the order of the groups as a rule: walk along it and look up the others
-    Py_ssize_t pos = 0;
-    PyObject *next_key = nullptr, *next_value = nullptr;
-    bool more = PyDict_Next(state, &pos, &next_key, &next_value);
+    Walk states(state);
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); ++i) {
         PyObject *obj = PyList_GET_ITEM(params, i);
         if (!THPVariable_Check(obj)) {
             PyErr_SetString(PyExc_TypeError, "adamw_step: a parameter is not a tensor");
             return nullptr;
         }
-        PyObject *st = nullptr;
-        if (more && next_key == obj) {
-            st = next_value;
-            more = PyDict_Next(state, &pos, &next_key, &next_value);
-        }
+        PyObject *st = states.next_if(obj);
         const at::Tensor &p = THPVariable_Unpack(obj);
         const at::Tensor &g = p.grad();
         if (!g.defined()) continue;
@@ -377,16 +390,29 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
             return nullptr;
         }
         if (!st) {
-            st = PyDict_GetItemWithError(state, obj);
+            st = states.find(obj);
             if (!st && PyErr_Occurred()) return nullptr;
         }
         if (!st || !PyDict_Check(st) || PyDict_GET_SIZE(st) == 0) {
             if (PyList_Append(missing, obj)) return nullptr;
             continue;
         }
+        Walk entries(st);
+        PyObject *count = entries.find(step_key);
+        if (!count || !THPVariable_Check(count)) {
+            if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, "step");
+            return nullptr;
+        }
+        const at::Tensor &c = THPVariable_Unpack(count);
+        if (!c.is_cpu() || c.scalar_type() != at::kFloat || c.numel() != 1) {
+            PyErr_Format(PyExc_ValueError, "%sstep is a host tensor of one fp32 number", kWho);
+            return nullptr;
+        }
+        float *count_ptr = c.data_ptr<float>();
+        const long long step = (long long)*count_ptr;
         void *s[4] = {nullptr, nullptr, nullptr, nullptr};
         for (Py_ssize_t k = 0; k < nkeys; ++k) {
-            PyObject *o = PyDict_GetItemWithError(st, PyTuple_GET_ITEM(keys, k));
+            PyObject *o = entries.find(PyTuple_GET_ITEM(keys, k));
             if (!o || !THPVariable_Check(o)) {
                 if (!PyErr_Occurred()) PyErr_Format(PyExc_KeyError, "%U", PyTuple_GET_ITEM(keys, k));
                 return nullptr;
@@ -401,24 +427,19 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
             }
             s[k] = t.data_ptr();
         }
-        PyObject *count = PyDict_GetItemWithError(st, step_key);
-        if (!count || !THPVariable_Check(count)) {
-            if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, "step");
-            return nullptr;
-        }
-        const at::Tensor &c = THPVariable_Unpack(count);
-        if (!c.is_cpu() || c.scalar_type() != at::kFloat || c.numel() != 1) {
-            PyErr_Format(PyExc_ValueError, "%sstep is a host tensor of one fp32 number", kWho);
-            return nullptr;
-        }
-        float *count_ptr = c.data_ptr<float>();
-        const long long step = (long long)*count_ptr;
         Batch *b = nullptr;
         for (Batch &x : batches)
             if (x.step == step && x.type == type && x.device == p.device()) b = &x;
         if (!b) {
             batches.push_back(Batch{p.device(), type, step, {}, {}, {}, {}, {}, {}});
             b = &batches.back();
+            const size_t most = (size_t)(PyList_GET_SIZE(params) - i);
+            b->p.reserve(most);
+            b->g.reserve(most);
+            for (auto &v : b->s) v.reserve(most);
+            b->n.reserve(most);
+            b->counts.reserve(most);
+            b->changed.reserve(most);
         }
         b->p.push_back(p.data_ptr());
         b->g.push_back(g.data_ptr());
