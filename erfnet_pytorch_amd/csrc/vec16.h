@@ -83,11 +83,14 @@ template <typename T> __device__ __forceinline__ u32x4 ld16(const T *p, int left
 // An access that leaves the caches to others (STREAM), or an ordinary one; V is a packed struct around a vector.
 template <bool STREAM, typename V> __device__ __forceinline__ auto ld_vec(const V *p)
 {
-    return STREAM ? __builtin_nontemporal_load(&p->v) : p->v;
+    typedef decltype(V::v) Loose __attribute__((aligned(alignof(V))));      // (a pointer to the member would promise its own)
+    if (STREAM) return (decltype(V::v))__builtin_nontemporal_load((const Loose *)p);
+    return p->v;
 }
 template <bool STREAM, typename V, typename R> __device__ __forceinline__ void st_vec(V *p, R r)
 {
-    if (STREAM) __builtin_nontemporal_store(r, &p->v);
+    typedef R Loose __attribute__((aligned(alignof(V))));
+    if (STREAM) __builtin_nontemporal_store((Loose)r, (Loose *)p);
     else p->v = r;
 }
 // The first `left` elements of f: 16 bytes, or the partial vector in pieces of 8, 4 and 2.
