@@ -16,9 +16,11 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <algorithm>
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/erfnet_hip.h"
@@ -467,6 +469,29 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     END_HANDLE_TH_ERRORS
 }
 
+// share_memory(list of tensors) -> whether two GPU tensors of it overlap (addresses are unique over the devices)
+PyObject *share_memory(PyObject *, PyObject *list)
+{
+    HANDLE_TH_ERRORS
+    if (!PyList_Check(list)) {
+        PyErr_SetString(PyExc_TypeError, "share_memory: (list)");
+        return nullptr;
+    }
+    std::vector<std::pair<const char *, size_t>> spans;
+    spans.reserve((size_t)PyList_GET_SIZE(list));
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+        PyObject *o = PyList_GET_ITEM(list, i);
+        if (!THPVariable_Check(o)) continue;
+        const Tensor &t = THPVariable_Unpack(o);
+        if (t.is_cuda() && t.numel()) spans.emplace_back((const char *)t.const_data_ptr(), t.nbytes());
+    }
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        if (spans[i - 1].first + spans[i - 1].second > spans[i].first) Py_RETURN_TRUE;
+    Py_RETURN_FALSE;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(name -> address): see Library
 PyObject *bind(PyObject *, PyObject *of)
 {
@@ -497,6 +522,7 @@ PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr},
                          {"layer_norm", (PyCFunction)(void (*)(void))layer_norm, METH_FASTCALL, nullptr},
                          {"log_probs", (PyCFunction)(void (*)(void))log_probs, METH_FASTCALL, nullptr},
                          {"adamw_step", (PyCFunction)(void (*)(void))adamw_step, METH_FASTCALL, nullptr},
+                         {"share_memory", share_memory, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -157,13 +157,6 @@ class SGD(torch.optim.Optimizer):
         return loss
 
 
-def _overlapping(params):
-    """Whether two GPU tensors of the list share memory (their updates run side by side)."""
-    spans = sorted((str(p.device), p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())
-                   for p in params if p.is_cuda and p.numel())
-    return any(a[0] == b[0] and b[1] < a[2] for a, b in zip(spans, spans[1:]))
-
-
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` (no amsgrad, no maximize) for fp32 and bf16 parameters, one launch per 90 tensors (66 with
     8-bit moments).
@@ -196,7 +189,7 @@ class AdamW(torch.optim.Optimizer):
         tensors = [p[1] if isinstance(p, tuple) else p for p in params]
         if len(set(map(id, tensors))) != len(params):
             raise ValueError("AdamW: a parameter appears twice in one group; its two updates would race")
-        if all(isinstance(p, torch.Tensor) for p in tensors) and _overlapping(tensors):
+        if any(getattr(p, "is_cuda", False) for p in tensors) and _lib.host().share_memory(tensors):
             raise ValueError("AdamW: two parameters of one group share memory; their updates would race")
         super().add_param_group({**param_group, "params": params})
 
@@ -251,7 +244,7 @@ class AdamW(torch.optim.Optimizer):
                     float(group["eps"]), float(group["weight_decay"]))
             first = host.adamw_step(*args)
             if first:                   # parameters that have their first gradient: nothing has been launched yet
-                if _overlapping(group["params"]):       # (they may have come to the GPU after the optimiser was made)
+                if host.share_memory(group["params"]):       # (they may have come to the GPU after the optimiser was made)
                     raise ValueError("AdamW: two parameters of one group share memory; their updates would race")
                 with torch.no_grad():
                     for p in first:
