@@ -28,27 +28,29 @@
 struct AdamwScalars {
     float b1, ob1, b2, ob2, keep, step, inv_root_c2, eps;       // ob = 1 - b, keep = 1 - lr wd, step = lr / c1
 };
-// The pointers of one launch's tensors, as many as 4 KB of kernel arguments hold.
+// One launch's tensors, as many as 4 KB of kernel arguments hold: 126 with 32-bit moments and 92 with 8-bit ones, by the 48 bits
+// that an address has (whole pointers and sizes: 90 and 66, and the 229 tensors of a network take a launch more).
+enum { ADAMW_P, ADAMW_G, ADAMW_M, ADAMW_V, ADAMW_MS, ADAMW_VS };        // 8 bits: codes of m and of the root, their scales
 template <int BITS> struct AdamwDesc {
-    static constexpr int MAX = 90;
+    static constexpr int POINTERS = BITS == 8 ? 6 : 4, MAX = BITS == 8 ? 92 : 126;
     AdamwScalars k;
     int count;
     unsigned end_chunk[MAX];    // running total of chunks up to and including tensor i
-    long long n[MAX];
-    void *p[MAX];
-    const void *g[MAX];
-    float *m[MAX], *v[MAX];
-};
-template <> struct AdamwDesc<8> {
-    static constexpr int MAX = 66;
-    AdamwScalars k;
-    int count;
-    unsigned end_chunk[MAX];
-    long long n[MAX];
-    void *p[MAX];
-    const void *g[MAX];
-    void *m[MAX], *r[MAX];      // codes of m and of the root
-    float *ms[MAX], *rs[MAX];   // their scales
+    unsigned last[MAX];         // elements in its last chunk
+    unsigned low[POINTERS][MAX], high[POINTERS / 2][MAX];       // high: two pointers' upper 16 bits
+    void set(int which, int i, const void *p)
+    {
+        const unsigned long long a = (unsigned long long)p;
+        unsigned &h = high[which / 2][i];
+        low[which][i] = (unsigned)a;
+        h = which & 1 ? (h & 0xffffu) | (unsigned)(a >> 32) << 16 : (h & 0xffff0000u) | (unsigned)(a >> 32);
+    }
+    // (by way of global memory's own pointers, or every access would be a flat one)
+    __device__ __forceinline__ char *get(int which, int t) const
+    {
+        const unsigned h = which & 1 ? high[which / 2][t] >> 16 : high[which / 2][t] & 0xffffu;
+        return (char *)(__attribute__((address_space(1))) char *)((unsigned long long)h << 32 | low[which][t]);
+    }
 };
 static_assert(sizeof(AdamwDesc<32>) <= 4096 && sizeof(AdamwDesc<8>) <= 4096, "kernel arguments");
 
@@ -191,6 +193,13 @@ struct AdamwCodes {
 template <typename T, int BITS, bool FULL, bool STREAM>
 __device__ __forceinline__ void adamw_chunk(const AdamwDesc<BITS> &d, int t, long long n, long long base)
 {
+    char *const pp = d.get(ADAMW_P, t), *const pm = d.get(ADAMW_M, t), *const pv = d.get(ADAMW_V, t);
+    const char *const pg = d.get(ADAMW_G, t);
+    float *pms = nullptr, *pvs = nullptr;
+    if constexpr (BITS == 8) {
+        pms = (float *)d.get(ADAMW_MS, t);
+        pvs = (float *)d.get(ADAMW_VS, t);
+    }
     const int lane = threadIdx.x & 63;
     f32x4 p[ADAMW_ROUNDS], g[ADAMW_ROUNDS], m[ADAMW_ROUNDS], v[ADAMW_ROUNDS];
     unsigned cm[ADAMW_ROUNDS], cr[ADAMW_ROUNDS];
@@ -199,17 +208,17 @@ __device__ __forceinline__ void adamw_chunk(const AdamwDesc<BITS> &d, int t, lon
     for (int r = 0; r < ADAMW_ROUNDS; ++r) {
         const long long at = base + (long long)r * ADAMW_BLOCK * 4, i = at + lane * 4;
         const int left = FULL ? 4 : n - i >= 4 ? 4 : n - i > 0 ? (int)(n - i) : 0;
-        p[r] = AdamwQuad<T>::template load<STREAM>(d.p[t], i, left);
-        g[r] = AdamwQuad<T>::template load<STREAM>(d.g[t], i, left);
+        p[r] = AdamwQuad<T>::template load<STREAM>(pp, i, left);
+        g[r] = AdamwQuad<T>::template load<STREAM>(pg, i, left);
         if constexpr (BITS == 32) {
-            m[r] = AdamwQuad<float>::load<STREAM>(d.m[t], i, left);
-            v[r] = AdamwQuad<float>::load<STREAM>(d.v[t], i, left);
+            m[r] = AdamwQuad<float>::load<STREAM>(pm, i, left);
+            v[r] = AdamwQuad<float>::load<STREAM>(pv, i, left);
         } else {
-            cm[r] = AdamwCodes::load<STREAM>(d.m[t], i, left);
-            cr[r] = AdamwCodes::load<STREAM>(d.r[t], i, left);
+            cm[r] = AdamwCodes::load<STREAM>(pm, i, left);
+            cr[r] = AdamwCodes::load<STREAM>(pv, i, left);
             const bool there = FULL || at < n;
-            ms[r] = there ? d.ms[t][at / ADAMW_SCALE_BLOCK] : 0.0f;
-            rs[r] = there ? d.rs[t][at / ADAMW_SCALE_BLOCK] : 0.0f;
+            ms[r] = there ? pms[at / ADAMW_SCALE_BLOCK] : 0.0f;
+            rs[r] = there ? pvs[at / ADAMW_SCALE_BLOCK] : 0.0f;
             m[r] = v[r] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};      // (what a block behind the last one counts for below)
         }
     }
@@ -230,10 +239,10 @@ __device__ __forceinline__ void adamw_chunk(const AdamwDesc<BITS> &d, int t, lon
             m[r][j] = mj;
             v[r][j] = BITS == 8 ? root : vj;
         }
-        AdamwQuad<T>::template store<false>(d.p[t], i, left, p[r]);
+        AdamwQuad<T>::template store<false>(pp, i, left, p[r]);
         if constexpr (BITS == 32) {
-            AdamwQuad<float>::store<STREAM>(d.m[t], i, left, m[r]);
-            AdamwQuad<float>::store<STREAM>(d.v[t], i, left, v[r]);
+            AdamwQuad<float>::store<STREAM>(pm, i, left, m[r]);
+            AdamwQuad<float>::store<STREAM>(pv, i, left, v[r]);
         }
     }
     if constexpr (BITS == 8) {
@@ -251,9 +260,9 @@ __device__ __forceinline__ void adamw_chunk(const AdamwDesc<BITS> &d, int t, lon
             if (!FULL && at >= n) break;
             float sm, sr;
             const unsigned nm = AdamwCodes::encode<false>(m[r], top[2 * r], sm), nr = AdamwCodes::encode<true>(v[r], top[2 * r + 1], sr);
-            AdamwCodes::store<STREAM>(d.m[t], i, left, nm);
-            AdamwCodes::store<STREAM>(d.r[t], i, left, nr);
-            if (lane == 0) { d.ms[t][at / ADAMW_SCALE_BLOCK] = sm; d.rs[t][at / ADAMW_SCALE_BLOCK] = sr; }
+            AdamwCodes::store<STREAM>(pm, i, left, nm);
+            AdamwCodes::store<STREAM>(pv, i, left, nr);
+            if (lane == 0) { pms[at / ADAMW_SCALE_BLOCK] = sm; pvs[at / ADAMW_SCALE_BLOCK] = sr; }
         }
     }
 }
@@ -266,7 +275,8 @@ __global__ __launch_bounds__(ADAMW_BLOCK) void adamw_kernel(const AdamwDesc<BITS
     const int t = __popcll(__ballot(lane < d.count && blockIdx.x >= d.end_chunk[l0])) +
                   __popcll(__ballot(lane + 64 < d.count && blockIdx.x >= d.end_chunk[l1]));
     const unsigned first = t ? d.end_chunk[t - 1] : 0u;
-    const long long n = d.n[t], chunk = (long long)(blockIdx.x - first) * ADAMW_CHUNK;
+    const long long n = (long long)(d.end_chunk[t] - first - 1u) * ADAMW_CHUNK + d.last[t];
+    const long long chunk = (long long)(blockIdx.x - first) * ADAMW_CHUNK;
     const long long base = chunk + (threadIdx.x >> 6) * ADAMW_SCALE_BLOCK;
     if (chunk + ADAMW_CHUNK <= n) adamw_chunk<T, BITS, true, STREAM>(d, t, n, base);
     else adamw_chunk<T, BITS, false, STREAM>(d, t, n, base);

@@ -358,6 +358,9 @@ int adamw_step(const char *what, int count, void *const *p, const void *const *g
         elements += numel[i];
         if (numel[i] && (!p[i] || !g[i] || !m[i] || !v[i] || (BITS == 8 && (!ms[i] || !vs[i]))))
             return fail("%s: tensor %d has a null pointer", what, i);
+        for (const void *a : {(const void *)p[i], g[i], (const void *)m[i], (const void *)v[i], BITS == 8 ? (const void *)ms[i] : nullptr,
+                              BITS == 8 ? (const void *)vs[i] : nullptr})
+            if ((unsigned long long)a >> 48) return fail("%s: tensor %d has an address of more than 48 bits", what, i);
         if (numel[i] / ADAMW_CHUNK >= (1ll << 31) - 1) return fail("%s: tensor %d is too large", what, i);
     }
     // a replayed launch would repeat this step's bias corrections
@@ -377,10 +380,9 @@ int adamw_step(const char *what, int count, void *const *p, const void *const *g
             const unsigned long long c = ((unsigned long long)numel[i] + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
             if (chunks + c >= (1ull << 31)) break;              // goes into the next launch
             const int k = d.count++;
-            d.p[k] = p[i]; d.g[k] = g[i];
-            if constexpr (BITS == 8) { d.m[k] = m[i]; d.r[k] = v[i]; d.ms[k] = ms[i]; d.rs[k] = vs[i]; }
-            else { d.m[k] = (float *)m[i]; d.v[k] = (float *)v[i]; }
-            d.n[k] = numel[i];
+            const void *const of[] = {p[i], g[i], m[i], v[i], BITS == 8 ? ms[i] : nullptr, BITS == 8 ? vs[i] : nullptr};
+            for (int w = 0; w < AdamwDesc<BITS>::POINTERS; ++w) d.set(w, k, of[w]);
+            d.last[k] = (unsigned)(numel[i] - (long long)(c - 1) * ADAMW_CHUNK);
             chunks += c;
             d.end_chunk[k] = (unsigned)chunks;
         }
