@@ -145,9 +145,9 @@ struct LogpShape {
     bool moved;                     // the class axis was brought to the end
 };
 
-// The results in the caller's shapes; what backward needs goes to kept: the logits as the kernels read them, the targets,
+// The results in the caller's shapes; what backward needs goes to kept, if it is wanted: the logits as the kernels read them, the targets,
 // the statistics, the entropy and the alternatives' indices as the kernels wrote them.
-variable_list logp_forward(const Tensor &logits, const Tensor &target0, LogpShape &s, variable_list &kept)
+variable_list logp_forward(const Tensor &logits, const Tensor &target0, LogpShape &s, variable_list *kept)
 {
     const int64_t nd = logits.dim();
     s.v = logits.size(s.axis);
@@ -168,7 +168,8 @@ variable_list logp_forward(const Tensor &logits, const Tensor &target0, LogpShap
         s.outer = pixels / s.inner;
         s.ld = 0;
     } else {
-        x = (s.moved ? logits.movedim(s.axis, -1) : logits).reshape({pixels, s.v});
+        x = s.moved ? logits.movedim(s.axis, -1) : logits;
+        if (nd != 2) x = x.reshape({pixels, s.v});
         s.outer = pixels;
         s.inner = 1;
         if (x.stride(1) != 1 || (pixels > 1 && x.stride(0) < s.v)) x = x.contiguous();
@@ -179,14 +180,15 @@ variable_list logp_forward(const Tensor &logits, const Tensor &target0, LogpShap
         else if (!s.moved) full.push_back(s.top_k);
     if (s.moved) full.push_back(s.top_k);
     const Tensor lp = fresh(target.sizes(), at::kFloat, x), ent = fresh(target.sizes(), at::kFloat, x);
-    const Tensor top = fresh(full, at::kFloat, x), idx = fresh(full, at::kLong, x), stats = fresh({2 * pixels}, at::kFloat, x);
-    Tensor ws;
+    const Tensor top = fresh(full, at::kFloat, x), idx = fresh(full, at::kLong, x);
+    Tensor stats, ws;
+    if (kept) stats = fresh({2 * pixels}, at::kFloat, x);
     const int64_t n_ws = (int64_t)lib.logp_ws(s.outer, (int)s.v, s.inner, (int)s.top_k);
     if (n_ws) ws = fresh({n_ws}, at::kByte, x);
     check(lib.logp_fwd[kind(x)](x.data_ptr(), (const long long *)target.data_ptr(), floats(lp), floats(ent), floats(stats), floats(top),
                                 (long long *)idx.data_ptr(), s.outer, (int)s.v, s.inner, s.ld, (int)s.top_k, s.ignore,
                                 ws.defined() ? ws.data_ptr() : nullptr, (size_t)n_ws, stream(x.device())));
-    kept = {x, target, stats, ent, idx};
+    if (kept) *kept = {x, target, stats, ent, idx};
     if (s.moved) return {lp, ent, top.movedim(-1, s.axis), idx.movedim(-1, s.axis)};
     return {lp, ent, top, idx};
 }
@@ -196,7 +198,7 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
                                  int64_t ignore, int64_t axis)
     {
         LogpShape s{0, 0, 0, 0, top_k, ignore, axis, false};
-        variable_list kept, out = logp_forward(logits, target0, s, kept);
+        variable_list kept, out = logp_forward(logits, target0, s, &kept);
         ctx->save_for_backward(kept);
         ctx->saved_data["shape"] = std::vector<int64_t>{s.outer, s.v, s.inner, s.ld, s.top_k, s.ignore, s.axis, s.moved};
         ctx->saved_data["logits"] = logits.sizes().vec();
@@ -275,8 +277,7 @@ PyObject *log_probs(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         out = LogProbs::apply(logits, target, top_k, ignore, axis);
     } else {
         LogpShape s{0, 0, 0, 0, top_k, ignore, axis, false};
-        variable_list kept;
-        out = logp_forward(logits, target, s, kept);
+        out = logp_forward(logits, target, s, nullptr);
     }
     THPObjectPtr tuple(PyTuple_New(4));
     if (!tuple) return nullptr;

@@ -24,7 +24,7 @@ struct LpDesc {
     const void *x;              // logits, storage type T
     const long long *target;    // [rows]
     float *log_prob, *entropy;  // [rows]
-    float2 *stats;              // [rows] (m, log S); log S = -infinity marks a row with no class
+    float2 *stats;              // [rows] (m, log S); log S = -infinity marks a row with no class.  Forward: may be null
     float *top_lp;              // row kernels [rows][k], pixel kernel [outer][k][inner]
     long long *top_idx;
     long long rows;             // row kernels: rows; pixel kernels: outer * inner
@@ -358,7 +358,7 @@ __device__ __forceinline__ void lp_write_row(const LpDesc &d, long long row, con
     const bool none = r.s == 0.0f;
     const float log_s = none ? -INFINITY : logf(r.s);
     if (lane == 0) {
-        d.stats[row] = make_float2(r.m, log_s);
+        if (d.stats) d.stats[row] = make_float2(r.m, log_s);
         d.entropy[row] = none ? 0.0f : log_s - r.a / r.s;
         const long long t = d.target[row];
         float lp = 0.0f;
@@ -675,7 +675,7 @@ __global__ __launch_bounds__(LP_BLOCK) void lp_pixels_kernel(const LpDesc d)
     }
     const bool none = r.s == 0.0f;
     const float log_s = none ? -INFINITY : logf(r.s);
-    d.stats[p] = make_float2(r.m, log_s);
+    if (d.stats) d.stats[p] = make_float2(r.m, log_s);
     d.entropy[p] = none ? 0.0f : log_s - r.a / r.s;
     const long long t = d.target[p];
     float lp = 0.0f;

@@ -240,7 +240,7 @@ int lp_forward(const void *x, const long long *target, float *log_prob, float *e
 {
     if (lp_check("log_probs", outer, V, inner, k)) return 1;
     if (outer == 0) return 0;
-    if (!x || !target || !log_prob || !entropy || !stats || (k && (!top_lp || !top_idx))) return fail("log_probs: null pointer");
+    if (!x || !target || !log_prob || !entropy || (k && (!top_lp || !top_idx))) return fail("log_probs: null pointer");
     if (inner == 1 && ld < V && outer > 1) return fail("log_probs: rows overlap (stride %lld, %d classes)", ld, V);
     LpDesc d;
     memset(&d, 0, sizeof(d));

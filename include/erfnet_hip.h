@@ -342,7 +342,7 @@ int erf_layer_norm_backward(const float *x, const float *w, const float *mean, c
  *   log_prob [outer][inner] = log p[target];  entropy [outer][inner] = -sum p log p;
  *   top_log_probs / top_indices [outer][top_k][inner]: the top_k largest, equal ones by index; top_k <= V and
  *   <= ERF_LOG_PROBS_MAX_TOP (inner = 1) or ERF_LOG_PROBS_MAX_TOP_PIXELS; both may be NULL for top_k = 0;
- *   stats [outer][inner][2]: maximum and log of the sum of exponentials above it, for backward.
+ *   stats [outer][inner][2]: maximum and log of the sum of exponentials above it, for backward; NULL if none follows.
  * Logits of -infinity have probability 0; a row of nothing else has log probabilities of -infinity, entropy 0 and no
  * gradient.  NaN or +infinity makes its row NaN.  ws: erf_log_probs_workspace_bytes().
  * Backward: g_log_prob, g_entropy [outer][inner] and g_top [outer][top_k][inner], each may be NULL (zero); dlogits is dense
