@@ -155,12 +155,13 @@ __global__ __launch_bounds__(LANES ? NORM_BLOCK : 1024) void norm_fwd_kernel(con
 // Backward, the same walk, from the last row to the first: what was read and written last is what the 256 MB cache
 // still has (8191 x 8192 bf16, forward and backward: 136 -> 131 us).  Every thread keeps the weight's and bias's gradient of its own channels in registers over
 // all rows it meets; the block's sums go to partial, and norm_grad_sum_kernel adds the blocks in order.
-// THREADS: most threads of a block kernel (0: wave kernel).  1024 of them have 128 registers each, which hold the sums
-// but neither the weight nor the next row's loads: AHEAD is off there.
+// THREADS: most threads of a block kernel (0: wave kernel).  Beyond 8192 channels bf16 takes 32 elements a thread, whose 256
+// registers hold the sums and the next row's loads, fp32 1024 threads with 128 registers for the sums alone; the weight is read again for
+// every row (4000 x 12000, 1024 / 512 threads: bf16 83 / 73 us, fp32 120 / 124).
 template <typename T, int R, int LANES, int THREADS, bool EVEN>
 __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kernel(const NormDesc d)
 {
-    constexpr bool BLOCK = THREADS != 0, AHEAD = THREADS != 1024;
+    constexpr bool BLOCK = THREADS != 0, HELD = THREADS != 1024 && R * Vec16<T>::N <= 16, AHEAD = THREADS != 1024;
     static_assert(BLOCK == (LANES == 0), "one of the two");
     constexpr int N = Vec16<T>::N;
     extern __shared__ float acc[];              // wave kernel: [4 waves][2][C]
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kerne
     float w[R][N], dw[R][N], db[R][N];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (AHEAD) norm_params<N, EVEN>(w[r], d.w, (r * threads + me) * N, C, 1.0f);
+        if (HELD) norm_params<N, EVEN>(w[r], d.w, (r * threads + me) * N, C, 1.0f);
 #pragma unroll
         for (int i = 0; i < N; ++i) dw[r][i] = db[r][i] = 0.0f;
     }
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kerne
             const int c = (r * threads + me) * N;
             norm_unpack<T, EVEN>(nx[r], h[r], C - c);
             norm_unpack<T, EVEN>(ng[r], g[r], C - c);         // zero beyond the row: nothing below counts it
-            if (!AHEAD) norm_params<N, EVEN>(w[r], d.w, c, C, 1.0f);
+            if (!HELD) norm_params<N, EVEN>(w[r], d.w, c, C, 1.0f);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 h[r][i] = (h[r][i] - mean) * rstd;

@@ -142,8 +142,10 @@ int norm_backward(const void *x, const float *w, const float *mean, const float 
         const size_t lds = params && p.wave ? (size_t)8 * C * sizeof(float) : 0;
         norm_by_shape<T>(p, C, [&](auto even, auto rounds, auto lanes) {
             if constexpr (lanes > 0) norm_bwd_kernel<T, rounds, lanes, 0, even><<<blocks, NORM_BLOCK, lds, st>>>(d);
-            else if (p.threads > 512) norm_bwd_kernel<T, rounds, 0, 1024, even><<<blocks, p.threads, 0, st>>>(d);
-            else norm_bwd_kernel<T, rounds, 0, 512, even><<<blocks, p.threads, 0, st>>>(d);
+            else if (p.threads <= 512) norm_bwd_kernel<T, rounds, 0, 512, even><<<blocks, p.threads, 0, st>>>(d);
+            else if constexpr (sizeof(T) == 2)
+                norm_bwd_kernel<T, 2 * rounds, 0, 512, even><<<blocks, (p.threads / 2 + 63) / 64 * 64, 0, st>>>(d);
+            else norm_bwd_kernel<T, rounds, 0, 1024, even><<<blocks, p.threads, 0, st>>>(d);
         });
         LAUNCHED("norm_bwd_kernel");
     }

@@ -75,7 +75,7 @@ def check_norm(got, x, gy, w, b, eps, what):
 
 
 NORM_SHAPES = [(1, 1), (3, 1), (1, 5), (33, 1000), (7, 16), (129, 17), (64, 31), (50, 64), (300, 128), (9, 255), (5, 1024),
-               (4, 1025), (3, 2047), (6, 4096), (2, 4097), (3, 8191), (2, 16384)]
+               (4, 1025), (3, 2047), (6, 4096), (2, 4097), (3, 8191), (2, 16384), (5, 8193), (300, 12001)]
 
 
 @gpu
