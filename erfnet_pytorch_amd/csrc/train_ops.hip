@@ -76,10 +76,11 @@ int norm_blocks(const NormPlan &p, long long rows, int threads, int turns)
     return (int)std::min(std::min(all, full), std::max<long long>(256, all / turns));
 }
 // (us: forward with 2048 / 1024 threads a unit, 8191 x 8192 bf16 47 / 43, 49152 x 128 fp32 9.3 / 9.6; backward, a wave a row, 1024
-// / 512, 20000 x 1000 fp32 54 / 50, 786432 x 16 bf16 20.6 / 19.2; a block a row, 1024 / 512 / 256, 8191 x 4096 bf16 67 / 51 / 47, 8191 x 8192 97 /
-// 86 / 86, 8191 x 2048 35 / 35 / 31)
+// / 512, 20000 x 1000 fp32 54 / 50, 786432 x 16 bf16 20.6 / 19.2; a block a row, 1024 / 512 / 256, 8191 x 4096 bf16 67 / 51 / 47,
+// 8191 x 8192 97 / 86 / 86, and 256 / 384, where 128 threads are three blocks instead of two and 192 two instead of one, 20000 x
+// 1030 64 / 51, 20000 x 2049 102 / 81, 20000 x 2048 55 / 56)
 #define NORM_FWD_BLOCKS(p, rows) norm_blocks(p, rows, 1024, 1)
-#define NORM_BWD_BLOCKS(p, rows) norm_blocks(p, rows, (p).wave ? 512 : 256, 8)
+#define NORM_BWD_BLOCKS(p, rows) norm_blocks(p, rows, (p).wave ? 512 : 384, 8)
 
 // (partial sums of wide rows, us with 16 / 64 columns a block: C = 2048 12.6 / 11.8, 4096 11.9 / 8.1, 8192 13.3 / 7.3; 16 below,
 // where 64 leave most compute units without a block)
