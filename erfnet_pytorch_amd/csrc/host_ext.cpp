@@ -61,17 +61,19 @@ Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const Tensor &beside, b
 Tensor parameter(const Tensor &t) { return t.defined() ? t.to(at::kFloat).contiguous() : t; }
 
 // What backward returns, from an operator whose gradient has none: where a graph of the backward pass is recorded
-// (`recorded`), the results hang on a node that raises, in front of everything that they depend on.
-variable_list first_order(variable_list grads, bool recorded, const variable_list &inputs)
+// (`recorded`), the results hang on a node that raises, in front of everything that they depend on: the upstream gradients,
+// and the inputs by the edges of the node that is running (the tensors it has saved may be copies and views of the inputs,
+// made without a graph: autograd would find no way from them to the inputs, and leave the node out).
+variable_list first_order(variable_list grads, bool recorded, const variable_list &upstream)
 {
     if (!recorded) return grads;
-    bool any = false;
-    for (const Tensor &t : inputs) any |= t.defined() && t.requires_grad();
-    if (!any) return grads;
+    torch::autograd::edge_list edges = torch::autograd::collect_next_edges(upstream);
+    if (const auto running = torch::autograd::get_current_node())
+        edges.insert(edges.end(), running->next_edges().begin(), running->next_edges().end());
+    if (std::none_of(edges.begin(), edges.end(), [](const torch::autograd::Edge &e) { return e.is_valid(); })) return grads;
     const at::AutoGradMode on(true);
     auto node = std::make_shared<torch::autograd::Error>(
-        "erfnet_pytorch_amd: the gradient of layer_norm / log_probs is not differentiable",
-        torch::autograd::collect_next_edges(inputs));
+        "erfnet_pytorch_amd: the gradient of layer_norm / log_probs is not differentiable", std::move(edges));
     for (Tensor &g : grads)
         if (g.defined()) torch::autograd::set_history(g, node);
     return grads;
@@ -135,7 +137,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                                     ws.defined() ? ws.data_ptr() : nullptr, (size_t)n_ws, stream(x.device())));
         if (dw.defined()) dw = dw.to(w.scalar_type());
         if (db.defined()) db = db.to((at::ScalarType)bias);
-        return first_order({dx, dw, db, Tensor(), Tensor()}, recorded, {x, w, grads[0]});
+        return first_order({dx, dw, db, Tensor(), Tensor()}, recorded, grads);
     }
 };
 
@@ -230,7 +232,7 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
                                     (const long long *)idx.data_ptr(), floats(g[0]), floats(g[1]), floats(g[2]), dx.data_ptr(),
                                     s[0], (int)s[1], s[2], s[3], (int)s[4], s[5], stream(x.device())));
         if (moved) dx = dx.movedim(-1, axis);
-        return first_order({dx, Tensor(), Tensor(), Tensor(), Tensor()}, recorded, {x, grads[0], grads[1], grads[2]});
+        return first_order({dx, Tensor(), Tensor(), Tensor(), Tensor()}, recorded, grads);
     }
 };
 

@@ -1,0 +1,79 @@
+"""Layer norm, token log probabilities and AdamW: calls off the ordinary path (other derivatives, tracing, threads, very many
+rows, state that arrives late), and bounds that leave no entry of a large result unchecked.  The formulas' references and
+the bounds' reasoning are those of test_train_ops.py."""
+import pytest
+import torch
+
+DEV = "cuda:0"
+gpu = pytest.mark.gpu
+
+
+def noise(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+# ================================================================================ derivatives
+def _norm_of(layout):
+    """x (a leaf) and y = layer_norm of a layout of it that the kernels read as it is, as a view, or as a copy."""
+    from erfnet_pytorch_amd import functional as hipf
+    if layout == "rows":
+        x = noise(6, 32)
+        return x, lambda t: hipf.layer_norm(t)
+    if layout == "transposed":
+        return noise(32, 6), lambda t: hipf.layer_norm(t.t())
+    if layout == "every other row":
+        return noise(12, 32), lambda t: hipf.layer_norm(t[::2])
+    if layout == "nchw":
+        return noise(2, 16, 3, 5), lambda t: hipf.layer_norm(t, dim=1)
+    assert layout == "nhwc"
+    return noise(2, 16, 3, 5).to(memory_format=torch.channels_last), lambda t: hipf.layer_norm(t, dim=1)
+
+
+def _logp_of(layout):
+    from erfnet_pytorch_amd import functional as hipf
+    shape, dim = {"rows": ((6, 32), -1), "tokens": ((2, 3, 32), -1), "one row": ((32,), 0), "moved axis": ((32, 6), 0),
+                  "pixels": ((2, 16, 3, 5), 1), "many classes": ((2, 80, 3, 5), 1)}[layout]
+    t = torch.zeros(shape[:dim] + shape[dim + 1:] if dim >= 0 else shape[:-1], dtype=torch.int64)
+    return noise(*shape), lambda x: hipf.log_probs(x, t.to(DEV), top_k=2, dim=dim)
+
+
+NORM_LAYOUTS = ["rows", "transposed", "every other row", "nchw", "nhwc"]
+LOGP_LAYOUTS = ["rows", "tokens", "one row", "moved axis", "pixels", "many classes"]
+
+
+def _second(f, x, out, extra):
+    """autograd.grad of the gradient, with an upstream gradient that is a constant: only the operator's inputs lead back."""
+    x = x.to(DEV).requires_grad_()
+    y = out(f(x))
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+    if extra:
+        dx = dx + x * x
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(dx, x, torch.ones_like(dx), allow_unused=True)
+
+
+@gpu
+@pytest.mark.parametrize("extra", [False, True])
+@pytest.mark.parametrize("layout", NORM_LAYOUTS)
+def test_second_derivative_of_layer_norm_raises_for_every_layout(layout, extra):
+    x, f = _norm_of(layout)
+    _second(f, x, lambda y: y, extra)
+
+
+@gpu
+@pytest.mark.parametrize("extra", [False, True])
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("layout", LOGP_LAYOUTS)
+def test_second_derivative_of_log_probs_raises_for_every_layout(layout, which, extra):
+    x, f = _logp_of(layout)
+    _second(f, x, lambda r: r[which], extra)
+
+
+@gpu
+def test_second_derivative_by_way_of_the_weight_raises():
+    from erfnet_pytorch_amd import functional as hipf
+    x, w = noise(2, 3, 16).to(DEV).requires_grad_(), noise(16, seed=1).to(DEV).requires_grad_()
+    y = hipf.layer_norm(x.transpose(0, 1), w)
+    dw, = torch.autograd.grad(y, w, torch.ones_like(y), create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(dw.sum(), x, allow_unused=True)
