@@ -77,3 +77,35 @@ def test_second_derivative_by_way_of_the_weight_raises():
     dw, = torch.autograd.grad(y, w, torch.ones_like(y), create_graph=True)
     with pytest.raises(RuntimeError, match="not differentiable"):
         torch.autograd.grad(dw.sum(), x, allow_unused=True)
+
+
+@gpu
+@pytest.mark.parametrize("leaf", [False, True])
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "logits"])
+def test_forward_mode_raises(which, leaf):
+    import torch.autograd.forward_ad as fwd
+    from erfnet_pytorch_amd import functional as hipf
+    t = {"x": noise(4, 16), "weight": noise(16, seed=1), "bias": noise(16, seed=2), "logits": noise(4, 16)}
+    t = {k: v.to(DEV).requires_grad_(leaf) for k, v in t.items()}
+    target = torch.zeros(4, dtype=torch.int64, device=DEV)
+    with fwd.dual_level():
+        t[which] = fwd.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            if which == "logits":
+                hipf.log_probs(t["logits"], target)
+            else:
+                hipf.layer_norm(t["x"], t["weight"], t["bias"])
+    hipf.log_probs(t["logits"].detach(), target)
+
+
+@gpu
+@pytest.mark.parametrize("op", ["layer_norm", "log_probs"])
+def test_forward_mode_over_the_gradient_raises(op):
+    import torch.autograd.forward_ad as fwd
+    from erfnet_pytorch_amd import functional as hipf
+    x = noise(4, 16).to(DEV).requires_grad_()
+    y = hipf.layer_norm(x) if op == "layer_norm" else hipf.log_probs(x, torch.zeros(4, dtype=torch.int64, device=DEV)).entropy
+    with fwd.dual_level():
+        g = fwd.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, x, g)
