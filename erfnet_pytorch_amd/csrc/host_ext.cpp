@@ -8,12 +8,14 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/object_ptr.h>
 
 #include <algorithm>
@@ -85,6 +87,14 @@ void no_tangents(const char *what, at::ArrayRef<Tensor> inputs)
     for (const Tensor &t : inputs)
         TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), "erfnet_pytorch_amd: ", what,
                                     " has no forward-mode derivative");
+}
+
+// A tracer sees nothing of calls past the dispatcher: the results would be constants of its graph.
+void no_tracing(const char *what)
+{
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() &&
+                                    !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+                                "erfnet_pytorch_amd: ", what, " cannot be traced");
 }
 
 // ---------------------------------------------------------------------------------------------- layer norm
@@ -267,6 +277,7 @@ PyObject *layer_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     const double eps = PyFloat_AsDouble(args[3]);
     const bool image = PyObject_IsTrue(args[4]);
     if (PyErr_Occurred()) return nullptr;
+    no_tracing("layer_norm");
     no_tangents("layer_norm", {x, w, b});
     auto given = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     if (wanted({x, w, b})) return THPVariable_Wrap(LayerNorm::apply(x, given(w), given(b), eps, image));
@@ -285,6 +296,7 @@ PyObject *log_probs(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     const Tensor logits = unpack(args[0]), target = unpack(args[1]);
     const int64_t top_k = PyLong_AsLongLong(args[2]), ignore = PyLong_AsLongLong(args[3]), axis = PyLong_AsLongLong(args[4]);
     if (PyErr_Occurred()) return nullptr;
+    no_tracing("log_probs");
     no_tangents("log_probs", {logits});
     variable_list out;
     if (wanted({logits})) {

@@ -109,3 +109,21 @@ def test_forward_mode_over_the_gradient_raises(op):
         g = fwd.make_dual(torch.ones_like(y), torch.ones_like(y))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(y, x, g)
+
+
+# ================================================================================ tracing
+@gpu
+@pytest.mark.parametrize("how", ["jit", "fx"])
+@pytest.mark.parametrize("op", ["layer_norm", "log_probs"])
+def test_tracing_raises(op, how):
+    """The results would be constants of the graph: the answer for the example's input, whatever comes."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from erfnet_pytorch_amd import functional as hipf
+    x, target = noise(4, 16).to(DEV), torch.zeros(4, dtype=torch.int64, device=DEV)
+
+    def f(t):
+        return hipf.layer_norm(t) if op == "layer_norm" else hipf.log_probs(t, target).log_prob
+
+    with pytest.raises(NotImplementedError, match="cannot be traced"):
+        torch.jit.trace(f, x) if how == "jit" else make_fx(f)(x)
+    f(x)
