@@ -202,12 +202,16 @@ __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kerne
             if (!HELD) norm_params<N, EVEN>(w[r], d.w, c, C, 1.0f);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                h[r][i] = (h[r][i] - mean) * rstd;
+                // (s1 without rstd: behind the row's end, where x and g are zero, 0 - mean in units of the row's spread may pass the
+                // type's range, and infinity times zero would be counted.  Differences are below 2^64 wherever fp32 holds their
+                // squares; where it does not, rstd is 0 and s1 with it.)
+                const float off = h[r][i] - mean;
+                h[r][i] = off * rstd;
                 dw[r][i] += g[r][i] * h[r][i];
                 db[r][i] += g[r][i];
                 g[r][i] *= w[r][i];
                 s0 += g[r][i];
-                s1 += g[r][i] * h[r][i];
+                s1 += g[r][i] * off;
             }
         }
         if (AHEAD && row + stride < d.rows) fetch(row + stride);
@@ -221,7 +225,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : NORM_BLOCK) void norm_bwd_kerne
             for (int i = 0; i < (int)(blockDim.x >> 6); ++i) { s0 += red[turn][0][i]; s1 += red[turn][1][i]; }
         }
         s0 *= inv_c;
-        s1 *= inv_c;
+        s1 = rstd > 0.0f ? s1 * (inv_c * rstd) : 0.0f;
         T *dx = (T *)d.y + (d.rows - 1 - row) * C;
 #pragma unroll
         for (int r = 0; r < R; ++r) {

@@ -127,3 +127,47 @@ def test_tracing_raises(op, how):
     with pytest.raises(NotImplementedError, match="cannot be traced"):
         torch.jit.trace(f, x) if how == "jit" else make_fx(f)(x)
     f(x)
+
+
+# ================================================================================ values
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("c", [3, 5, 20, 100, 1001, 1030, 5000, 12001, 12004])
+def test_layer_norm_gradient_of_high_rows_does_not_overflow_behind_their_end(c, kind):
+    """x = 2^113 everywhere: every partial sum is a multiple of it below 2^24 of them, so mean = x and xhat = 0 exactly, and
+    dx = (g w - mean(g w)) / sqrt(eps), dw = 0.  mean / sqrt(eps) = 2^113 1e5 is beyond fp32: it must not turn up where a
+    vector or a wave reaches beyond the row.  Errors: eps in fp32, root and product (under 8 u), the mean of g w (64 u of the
+    mean magnitude), dx's own rounding."""
+    from erfnet_pytorch_amd import functional as hipf
+    u, rows, eps = 2.0 ** -24, 5, 1e-10
+    g, w = noise(rows, c, seed=c, dtype=kind), 1 + 0.3 * noise(c, seed=c + 1)
+    x = torch.full((rows, c), 2.0 ** 113, dtype=kind).to(DEV).requires_grad_()
+    wd = w.to(DEV).requires_grad_()
+    dx, dw = torch.autograd.grad(hipf.layer_norm(x, wd, eps=eps), (x, wd), g.to(DEV))
+    gw = g.double() * w.double()
+    ref = (gw - gw.mean(1, keepdim=True)) / eps ** 0.5
+    size = (gw.abs() + gw.abs().mean(1, keepdim=True)) / eps ** 0.5
+    own = 0.0 if kind == torch.float32 else 2.0 ** -8
+    off = (dx.cpu().double() - ref).abs() - (72 * u * size * (1 + own) + own * ref.abs())
+    assert torch.isfinite(dx).all() and float(off.max()) <= 0
+    assert not dw.any()
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("c", [20, 1001, 5000, 12001])
+def test_layer_norm_of_a_row_whose_spread_is_beyond_fp32(c, kind):
+    """One entry of the type's lowest value: the squares sum to infinity, 1 / sqrt(var + eps) is 0, so y = bias and dx = 0, for
+    gradients whose product with the row is beyond fp32 too.  The other rows do not notice."""
+    from erfnet_pytorch_amd import functional as hipf
+    x, g, b = noise(4, c, seed=c, dtype=kind), 30 * noise(4, c, seed=c + 1, dtype=kind), noise(c, seed=c + 2)
+    plain = [t.to(DEV).requires_grad_() for t in (x, b)]
+    x = x.clone()
+    x[1, 3] = torch.finfo(kind).min
+    marked = [t.to(DEV).requires_grad_() for t in (x, b)]
+    (y0, (dx0, _)), (y, (dx, db)) = (
+        (y, torch.autograd.grad(y, t, g.to(DEV))) for t in (plain, marked) for y in [hipf.layer_norm(t[0], None, t[1])])
+    assert torch.equal(y[1], b.to(DEV).to(kind)) and not dx[1].any()
+    others = [0, 2, 3]
+    assert torch.equal(y[others], y0[others]) and torch.equal(dx[others], dx0[others])
+    assert torch.isfinite(db).all()
