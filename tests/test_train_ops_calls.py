@@ -171,3 +171,43 @@ def test_layer_norm_of_a_row_whose_spread_is_beyond_fp32(c, kind):
     others = [0, 2, 3]
     assert torch.equal(y[others], y0[others]) and torch.equal(dx[others], dx0[others])
     assert torch.isfinite(db).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("c", [1, 3, 13, 100, 1000, 1030, 8192, 12000, 16384])
+def test_layer_norm_of_constant_rows_is_the_bias(c, kind):
+    """Equal values, whose sum fp32 has to round: the differences from the first mean are all the same few units in the last
+    place, k of them, so their sum and the sum of their squares are exact below 2^24 units (c k^2), and what is left is zero."""
+    from erfnet_pytorch_amd import functional as hipf
+    levels = torch.tensor([0.1, 10.3, -1000.1, 1.7, 3.3e-7, 1.1e7, 0.0, 1e30])
+    x = levels[:, None].repeat(1, c).to(kind).to(DEV).requires_grad_()
+    w, b = noise(c, seed=1).to(DEV).requires_grad_(), noise(c, seed=2).to(DEV).requires_grad_()
+    y = hipf.layer_norm(x, w, b)
+    assert torch.equal(y, b.to(kind).expand_as(y))
+    g = noise(len(levels), c, seed=3, dtype=kind).to(DEV)
+    dx, dw = torch.autograd.grad(y, (x, w), g)
+    assert not dw.any()                                     # mean = x: xhat is zero in backward too
+    # rstd = 1 / sqrt(eps): eps in fp32, root, products (8 u); mean of g w: 64 u of its magnitudes
+    gw = g.double() * w.detach().double()
+    root = 1e-5 ** -0.5
+    ref, size = (gw - gw.mean(1, keepdim=True)) * root, (gw.abs() + gw.abs().mean(1, keepdim=True)) * root
+    own = 0.0 if kind == torch.float32 else 2.0 ** -8
+    assert float(((dx.double() - ref).abs() - 72 * 2.0 ** -24 * size * (1 + own) - own * ref.abs()).max()) <= 0
+
+
+@gpu
+@pytest.mark.parametrize("c", [100, 1000, 8192, 12000])
+def test_layer_norm_error_goes_with_the_spread_and_not_with_the_level(c):
+    """Level 1000, spread 0.01.  The differences from the first mean are exact (neighbouring floats), and that mean is off by at
+    most 48 u 1000 = 0.3 spreads.  What is left of the differences' mean errs by 64 u of their mean magnitude (below 1.3
+    spreads), the variance by 64 u (1 + 0.3^2) of itself, xhat by half of that and a few roundings of its own."""
+    from erfnet_pytorch_amd import functional as hipf
+    u = 2.0 ** -24
+    x, w, b = 1000 + 0.01 * noise(50, c, seed=c), 1 + 0.3 * noise(c, seed=1), 0.3 * noise(c, seed=2)
+    y = hipf.layer_norm(*(t.to(DEV) for t in (x, w, b)), eps=1e-12).cpu().double()
+    d = x.double() - x.double().mean(1, keepdim=True)
+    h = d / torch.sqrt((d * d).mean(1, keepdim=True) + 1e-12)
+    ref = h * w.double() + b.double()
+    bound = u * (w.double().abs() * (1.3 * 64 + h.abs() * (1.1 * 32 + 16)) + 4 * b.double().abs())
+    assert float(((y - ref).abs() / bound).max()) <= 1
