@@ -20,6 +20,9 @@ namespace {
         if (host_launched(name)) return 1;                                                         \
     } while (0)
 
+// HIP takes fewer than 2^32 threads in a launch: more work goes in several.
+long long most_blocks(int threads) { return ((1ll << 32) - 1) / threads; }
+
 int log2_up(int v)
 {
     int b = 0;
@@ -222,17 +225,46 @@ size_t lp_ws(long long outer, int V, long long inner, int k)
     return p.splits > 1 ? (size_t)outer * p.splits * (sizeof(float4) + (size_t)k * 8) : 0;
 }
 
+// The images or rows of d from `from` on, `n` of them.
+template <typename T> LpDesc lp_part(LpDesc d, long long from, long long n)
+{
+    const long long rows = from * d.inner, gathered = rows * d.k, group = d.inner > 1 ? d.V * d.inner : d.ld;
+    auto move = [](auto *&p, long long by) { if (p) p += by; };
+    d.x = (const T *)d.x + from * group;
+    d.target += rows;
+    move(d.log_prob, rows);
+    move(d.entropy, rows);
+    move(d.stats, rows);
+    move(d.top_lp, gathered);
+    move(d.top_idx, gathered);
+    move(d.g_lp, rows);
+    move(d.g_h, rows);
+    move(d.g_top, gathered);
+    if (d.dx) d.dx = (T *)d.dx + rows * d.V;
+    d.rows = n * d.inner;
+    return d;
+}
+// launch(part) over `outer` images or rows, at most `most` of them at a time; backward comes to the last first, as its kernels do.
+template <typename T, typename F>
+int lp_launch(const char *kernel, const LpDesc &d, long long outer, long long most, bool backward, F launch)
+{
+    for (long long done = 0; done < outer; done += most) {
+        const long long n = std::min(most, outer - done);
+        launch(lp_part<T>(d, backward ? outer - done - n : done, n));
+        LAUNCHED(kernel);
+    }
+    return 0;
+}
+#define LP_MOST_PIXELS (most_blocks(LP_BLOCK) * LP_BLOCK)
+
 int lp_check(const char *what, long long outer, int V, long long inner, int k)
 {
     if (outer < 0 || inner < 1) return fail("%s: negative or empty extent", what);
     if (V < 1 || V > LP_MAX_CLASSES) return fail("%s: 1..%d classes (got %d)", what, LP_MAX_CLASSES, V);
     const int most = inner > 1 ? ERF_LOG_PROBS_MAX_TOP_PIXELS : ERF_LOG_PROBS_MAX_TOP;
     if (k < 0 || k > most || k > V) return fail("%s: top_k must be in 0..%d and at most the class count (got %d)", what, most, k);
-    // one block per 256 pixels or per (row, segment): the grid must fit 31 bits
-    if (outer > (1ll << 40) / inner) return fail("%s: too many rows", what);
-    const long long blocks = inner > 1 ? (outer * inner + LP_BLOCK - 1) / LP_BLOCK
-                                       : outer * ((V + LP_BACKWARD_SEGMENT - 1) / LP_BACKWARD_SEGMENT);
-    if (blocks >= (1ll << 31)) return fail("%s: too many rows", what);
+    if (outer > (1ll << 39) / inner) return fail("%s: too many rows", what);
+    if (inner > LP_MOST_PIXELS) return fail("%s: more than %lld pixels an image", what, LP_MOST_PIXELS);
     return 0;
 }
 
@@ -253,14 +285,14 @@ int lp_forward(const void *x, const long long *target, float *log_prob, float *e
     if (lp_by_thread(outer, V, inner, k)) {
         d.group = inner > 1 ? V * inner : ld;
         d.next = inner;
-        const unsigned blocks = (unsigned)((d.rows + LP_BLOCK - 1) / LP_BLOCK);
-        if (k == 0) lp_pixels_kernel<T, 0><<<blocks, LP_BLOCK, 0, st>>>(d);
-        else if (k == 1) lp_pixels_kernel<T, 1><<<blocks, LP_BLOCK, 0, st>>>(d);
-        else if (k == 2) lp_pixels_kernel<T, 2><<<blocks, LP_BLOCK, 0, st>>>(d);
-        else if (k <= 4) lp_pixels_kernel<T, 4><<<blocks, LP_BLOCK, 0, st>>>(d);
-        else lp_pixels_kernel<T, 8><<<blocks, LP_BLOCK, 0, st>>>(d);
-        LAUNCHED("lp_pixels_kernel");
-        return 0;
+        return lp_launch<T>("lp_pixels_kernel", d, outer, LP_MOST_PIXELS / inner, false, [&](const LpDesc &d) {
+            const unsigned blocks = (unsigned)((d.rows + LP_BLOCK - 1) / LP_BLOCK);
+            if (k == 0) lp_pixels_kernel<T, 0><<<blocks, LP_BLOCK, 0, st>>>(d);
+            else if (k == 1) lp_pixels_kernel<T, 1><<<blocks, LP_BLOCK, 0, st>>>(d);
+            else if (k == 2) lp_pixels_kernel<T, 2><<<blocks, LP_BLOCK, 0, st>>>(d);
+            else if (k <= 4) lp_pixels_kernel<T, 4><<<blocks, LP_BLOCK, 0, st>>>(d);
+            else lp_pixels_kernel<T, 8><<<blocks, LP_BLOCK, 0, st>>>(d);
+        });
     }
     const LpPlan p = lp_plan<T>(outer, V, k);
     d.splits = p.splits; d.seg = p.seg;
@@ -269,16 +301,20 @@ int lp_forward(const void *x, const long long *target, float *log_prob, float *e
         d.part = (float4 *)ws;
         d.part_keys = (unsigned long long *)((char *)ws + (size_t)outer * p.splits * sizeof(float4));
     }
-    if (p.wave) {
-        const unsigned blocks = (unsigned)((outer + 3) / 4);
-        if (k) lp_rows_kernel<T, 64, true><<<blocks, LP_BLOCK, 0, st>>>(d);
-        else lp_rows_kernel<T, 64, false><<<blocks, LP_BLOCK, 0, st>>>(d);
-    } else {
-        const unsigned blocks = (unsigned)(outer * p.splits);
-        if (k) lp_rows_kernel<T, 256, true><<<blocks, LP_BLOCK, 0, st>>>(d);
-        else lp_rows_kernel<T, 256, false><<<blocks, LP_BLOCK, 0, st>>>(d);
-    }
-    LAUNCHED("lp_rows_kernel");
+    // (a row that is split is one of few: they go in one launch, and so does their join)
+    const long long most = p.wave ? most_blocks(LP_BLOCK) * 4 : most_blocks(LP_BLOCK) / p.splits;
+    const int rc = lp_launch<T>("lp_rows_kernel", d, outer, most, false, [&](const LpDesc &d) {
+        if (p.wave) {
+            const unsigned blocks = (unsigned)((d.rows + 3) / 4);
+            if (k) lp_rows_kernel<T, 64, true><<<blocks, LP_BLOCK, 0, st>>>(d);
+            else lp_rows_kernel<T, 64, false><<<blocks, LP_BLOCK, 0, st>>>(d);
+        } else {
+            const unsigned blocks = (unsigned)(d.rows * p.splits);
+            if (k) lp_rows_kernel<T, 256, true><<<blocks, LP_BLOCK, 0, st>>>(d);
+            else lp_rows_kernel<T, 256, false><<<blocks, LP_BLOCK, 0, st>>>(d);
+        }
+    });
+    if (rc) return rc;
     if (p.splits > 1) {
         if (p.splits <= 8) lp_join_kernel<T, 1><<<(unsigned)((outer + 3) / 4), LP_BLOCK, 0, st>>>(d);
         else lp_join_kernel<T, 16><<<(unsigned)outer, 1024, 0, st>>>(d);
@@ -304,30 +340,30 @@ int lp_backward(const void *x, const long long *target, const float *entropy, co
     if (inner > 1) {
         d.group = V * inner;
         d.next = inner;
-        const unsigned blocks = (unsigned)((d.rows + LP_BLOCK - 1) / LP_BLOCK);
-        lp_streamed(stream, [&](auto stream) {
-            if (!g_top || k == 0) lp_pixels_bwd_kernel<T, 0, stream><<<blocks, LP_BLOCK, 0, st>>>(d);
-            else if (k <= 2) lp_pixels_bwd_kernel<T, 2, stream><<<blocks, LP_BLOCK, 0, st>>>(d);
-            else lp_pixels_bwd_kernel<T, 8, stream><<<blocks, LP_BLOCK, 0, st>>>(d);
-        });
-        LAUNCHED("lp_pixels_bwd_kernel");
-        return 0;
-    }
-    if (V <= LP_SHORT && outer >= LP_SHORT_BACKWARD * V) {
-        lp_short_rows_bwd_kernel<T><<<(unsigned)((outer + LP_SHORT_ROWS - 1) / LP_SHORT_ROWS), LP_BLOCK, 0, st>>>(d);
-    } else if (V <= LP_WAVE_BACKWARD) {
-        lp_streamed(stream, [&](auto stream) {
-            lp_rows_bwd_kernel<T, 64, stream><<<(unsigned)((outer + 3) / 4), LP_BLOCK, 0, st>>>(d);
-        });
-    } else {
-        d.seg = LP_BACKWARD_SEGMENT;
-        d.splits = (V + d.seg - 1) / d.seg;
-        lp_streamed(stream, [&](auto stream) {
-            lp_rows_bwd_kernel<T, 256, stream><<<(unsigned)(outer * d.splits), LP_BLOCK, 0, st>>>(d);
+        return lp_launch<T>("lp_pixels_bwd_kernel", d, outer, LP_MOST_PIXELS / inner, true, [&](const LpDesc &d) {
+            const unsigned blocks = (unsigned)((d.rows + LP_BLOCK - 1) / LP_BLOCK);
+            lp_streamed(stream, [&](auto stream) {
+                if (!g_top || k == 0) lp_pixels_bwd_kernel<T, 0, stream><<<blocks, LP_BLOCK, 0, st>>>(d);
+                else if (k <= 2) lp_pixels_bwd_kernel<T, 2, stream><<<blocks, LP_BLOCK, 0, st>>>(d);
+                else lp_pixels_bwd_kernel<T, 8, stream><<<blocks, LP_BLOCK, 0, st>>>(d);
+            });
         });
     }
-    LAUNCHED("lp_rows_bwd_kernel");
-    return 0;
+    const bool by_elements = V <= LP_SHORT && outer >= LP_SHORT_BACKWARD * V, wave = V <= LP_WAVE_BACKWARD;
+    d.seg = LP_BACKWARD_SEGMENT;
+    d.splits = (V + d.seg - 1) / d.seg;
+    const long long most = by_elements ? most_blocks(LP_BLOCK) * LP_SHORT_ROWS
+                                       : wave ? most_blocks(LP_BLOCK) * 4 : most_blocks(LP_BLOCK) / d.splits;
+    return lp_launch<T>("lp_rows_bwd_kernel", d, outer, most, true, [&](const LpDesc &d) {
+        if (by_elements) {
+            lp_short_rows_bwd_kernel<T><<<(unsigned)((d.rows + LP_SHORT_ROWS - 1) / LP_SHORT_ROWS), LP_BLOCK, 0, st>>>(d);
+            return;
+        }
+        lp_streamed(stream, [&](auto stream) {
+            if (wave) lp_rows_bwd_kernel<T, 64, stream><<<(unsigned)((d.rows + 3) / 4), LP_BLOCK, 0, st>>>(d);
+            else lp_rows_bwd_kernel<T, 256, stream><<<(unsigned)(d.rows * d.splits), LP_BLOCK, 0, st>>>(d);
+        });
+    });
 }
 
 // ================================================================================ AdamW

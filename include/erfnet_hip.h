@@ -337,7 +337,7 @@ int erf_layer_norm_backward(const float *x, const float *w, const float *mean, c
 /* ---- Log probabilities of given classes, entropy and likeliest alternatives of a softmax (beside
  * erf_cross_entropy_forward, which returns only their mean over pixels) --------------------------------------------------
  * logits: [outer][V][inner].  inner = 1: rows of V contiguous classes, row_stride elements apart (>= V); inner > 1: dense,
- * the NCHW pixel layout (row_stride is ignored).  target: int64 [outer][inner]; a label that is ignore_index or outside
+ * the NCHW pixel layout (row_stride is ignored), inner < 2^32 - 255.  target: int64 [outer][inner]; a label that is ignore_index or outside
  * [0, V) gets log_prob 0 and passes no gradient.
  *   log_prob [outer][inner] = log p[target];  entropy [outer][inner] = -sum p log p;
  *   top_log_probs / top_indices [outer][top_k][inner]: the top_k largest, equal ones by index; top_k <= V and

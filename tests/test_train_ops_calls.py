@@ -211,3 +211,26 @@ def test_layer_norm_error_goes_with_the_spread_and_not_with_the_level(c):
     ref = h * w.double() + b.double()
     bound = u * (w.double().abs() * (1.3 * 64 + h.abs() * (1.1 * 32 + 16)) + 4 * b.double().abs())
     assert float(((y - ref).abs() / bound).max()) <= 1
+
+
+# ================================================================================ sizes
+@gpu
+def test_log_probs_of_more_rows_than_a_launch_of_backward_holds():
+    """2^24 + 12288 rows of 1025 bf16 classes (34 GB, and as much of a gradient): backward's blocks are more than HIP takes at once.
+    The rows repeat every 4096, which begin at the same place of a cache line, so the results repeat bit for bit."""
+    from erfnet_pytorch_amd import functional as hipf
+    tile, times, v = 4096, 4099, 1025
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("needs 90 GB")
+    piece, target = noise(tile, v, seed=5, dtype=torch.bfloat16).to(DEV), (torch.arange(tile) % v).to(DEV)
+    g = noise(tile, seed=6).to(DEV)
+    p = piece.clone().requires_grad_()
+    few = hipf.log_probs(p, target, top_k=2)
+    dp, = torch.autograd.grad((few.log_prob, few.entropy), p, (g, g))
+    x = piece.repeat(times, 1).requires_grad_()
+    r = hipf.log_probs(x, target.repeat(times), top_k=2)
+    for a, b in zip(r, few):
+        assert bool((a.detach().view(times, *b.shape) == b.detach()).all())
+    dx, = torch.autograd.grad((r.log_prob, r.entropy), x, (g.repeat(times), g.repeat(times)))
+    for part in dx.view(times, tile, v).split(256):
+        assert bool((part == dp).all())
