@@ -394,13 +394,13 @@ int adamw_step(const char *what, int count, void *const *p, const void *const *g
     long long elements = 0;
     for (int i = 0; i < count; ++i) {
         if (numel[i] < 0) return fail("%s: tensor %d has a negative size", what, i);
+        if (numel[i] >> 48) return fail("%s: tensor %d is too large", what, i);
         elements += numel[i];
         if (numel[i] && (!p[i] || !g[i] || !m[i] || !v[i] || (BITS == 8 && (!ms[i] || !vs[i]))))
             return fail("%s: tensor %d has a null pointer", what, i);
         for (const void *a : {(const void *)p[i], g[i], (const void *)m[i], (const void *)v[i], BITS == 8 ? (const void *)ms[i] : nullptr,
                               BITS == 8 ? (const void *)vs[i] : nullptr})
             if ((unsigned long long)a >> 48) return fail("%s: tensor %d has an address of more than 48 bits", what, i);
-        if (numel[i] / ADAMW_CHUNK >= (1ll << 31) - 1) return fail("%s: tensor %d is too large", what, i);
     }
     // a replayed launch would repeat this step's bias corrections
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
@@ -410,22 +410,37 @@ int adamw_step(const char *what, int count, void *const *p, const void *const *g
         return fail("%s: the step cannot be captured into a graph", what);
     }
     const bool stream = elements >= ADAMW_STREAM / (2 * (long long)sizeof(T) + (BITS == 8 ? 2 : 8));
+    const long long most = most_blocks(ADAMW_BLOCK);
     int i = 0;
+    long long done = 0;             // elements of tensor i that earlier launches have taken: whole chunks, and so whole scale blocks
     while (i < count) {
         d.count = 0;
-        unsigned long long chunks = 0;
-        for (; i < count && d.count < AdamwDesc<BITS>::MAX; ++i) {
-            if (numel[i] == 0) continue;
-            const unsigned long long c = ((unsigned long long)numel[i] + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
-            if (chunks + c >= (1ull << 31)) break;              // goes into the next launch
-            const int k = d.count++;
-            const void *const of[] = {p[i], g[i], m[i], v[i], BITS == 8 ? ms[i] : nullptr, BITS == 8 ? vs[i] : nullptr};
-            for (int w = 0; w < AdamwDesc<BITS>::POINTERS; ++w) d.set(w, k, of[w]);
-            d.last[k] = (unsigned)(numel[i] - (long long)(c - 1) * ADAMW_CHUNK);
-            chunks += c;
-            d.end_chunk[k] = (unsigned)chunks;
+        long long chunks = 0;
+        while (i < count && d.count < AdamwDesc<BITS>::MAX && chunks < most) {
+            const long long n = std::min(numel[i] - done, (most - chunks) * ADAMW_CHUNK);
+            if (n) {
+                const int k = d.count++;
+                const long long c = (n + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
+                auto from = [](const void *p, long long bytes) { return (const char *)p + bytes; };
+                d.set(ADAMW_P, k, from(p[i], done * (long long)sizeof(T)));
+                d.set(ADAMW_G, k, from(g[i], done * (long long)sizeof(T)));
+                d.set(ADAMW_M, k, from(m[i], BITS == 8 ? done : done * 4));
+                d.set(ADAMW_V, k, from(v[i], BITS == 8 ? done : done * 4));
+                if constexpr (BITS == 8) {
+                    d.set(ADAMW_MS, k, from(ms[i], done / ADAMW_SCALE_BLOCK * 4));
+                    d.set(ADAMW_VS, k, from(vs[i], done / ADAMW_SCALE_BLOCK * 4));
+                }
+                d.last[k] = (unsigned)(n - (c - 1) * ADAMW_CHUNK);
+                chunks += c;
+                d.end_chunk[k] = (unsigned)chunks;
+                done += n;
+            }
+            if (done == numel[i]) {
+                ++i;
+                done = 0;
+            }
         }
-        if (d.count == 0) continue;
+        if (d.count == 0) break;
         if (stream) adamw_kernel<T, BITS, true><<<(unsigned)chunks, ADAMW_BLOCK, 0, st>>>(d);
         else adamw_kernel<T, BITS, false><<<(unsigned)chunks, ADAMW_BLOCK, 0, st>>>(d);
         LAUNCHED("adamw_kernel");

@@ -145,3 +145,59 @@ def test_log_probs_of_any_number_of_rows_are_launched_within_hips_bounds(tmp_pat
 def test_log_probs_of_an_image_beyond_one_launch_are_refused(tmp_path):
     rc, rc2, why, forward, backward = run(tmp_path, 168, LOG_PROBS, 1, 2, (1 << 32) - 200, 1, 2)
     assert rc and rc2 and "pixels an image" in why and not forward and not backward
+
+
+ADAMW = r"""
+bits, size = int(sys.argv[3]), int(sys.argv[4])
+sizes = json.loads(sys.argv[5])
+count, most = len(sizes), 92 if bits == 8 else 126
+names = ["p", "g", "m", "ms", "v", "vs"] if bits == 8 else ["p", "g", "m", "v"]
+step = dict(p=size, g=size, m=1 if bits == 8 else 4, v=1 if bits == 8 else 4, ms=4 / 256, vs=4 / 256)
+room = (1 << 47) // (6 * count)         # of one tensor's table entry
+base = {n: [(j * count + i) * room + 256 for i in range(count)] for j, n in enumerate(names)}
+table = {n: (vp * count)(*base[n]) for n in names}
+name = "erf_adamw8_step" if bits == 8 else "erf_adamw_step"
+rc = getattr(lib, name + ("_bf16" if size == 2 else ""))(
+    count, *[table[n] for n in names], (ll * count)(*sizes), C.c_double(1e-3), C.c_double(0.9), C.c_double(0.999), C.c_double(1e-8),
+    C.c_double(0.01), ll(1), None)
+pointers = ["p", "g", "m", "v", "ms", "vs"][:len(names)]
+out = []
+for grid, raw in launches():        # AdamwDesc: 8 floats, count, end_chunk, last, low halves, pairs of upper 16 bits
+    n, = struct.unpack("i", raw[32:36])
+    u = struct.unpack(f"{most * (2 + len(names) + len(names) // 2)}I", raw[36:36 + 4 * most * (2 + len(names) + len(names) // 2)])
+    part = lambda j: u[j * most:(j + 1) * most]
+    end, last = part(0), part(1)
+    for t in range(n):
+        first = end[t - 1] if t else 0
+        elements = (end[t] - first - 1) * 2048 + last[t]
+        at = {}
+        for j, name in enumerate(pointers):
+            high = part(2 + len(names) + j // 2)[t] >> (16 * (j & 1)) & 0xffff
+            at[name] = high << 32 | part(2 + j)[t]
+        i = max(k for k in range(count) if base["p"][k] <= at["p"])
+        begin = (at["p"] - base["p"][i]) // size
+        moved = all(at[n] - base[n][i] == begin * s for n, s in ((n, step[n]) for n in names))
+        out.append([i, begin, elements, bool(moved)])
+    out.append([grid[0], grid[3], end[n - 1]])
+print(json.dumps([rc, lib.erf_last_error().decode(), out]))
+"""
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("size", [2, 4])
+@pytest.mark.parametrize("sizes", [
+    [7], [100] * 229, [0, 5, 0, 2048, 0], [35_000_000_000], [10, 34_359_738_367 * 3, 2049], [20_000_000_000, 20_000_000_000, 3],
+    [(2 ** 24 - 1) * 2048, 5], [(2 ** 24 - 1) * 2048 - 1, 5], [(2 ** 24 - 1) * 2048 + 1, 5]], ids=lambda s: f"{len(s)}x{max(s)}")
+def test_adamw_of_any_number_of_elements_is_launched_within_hips_bounds(tmp_path, sizes, size, bits):
+    rc, why, out = run(tmp_path, 4096, ADAMW, bits, size, json.dumps(sizes))
+    assert rc == 0, why
+    launches, parts = [o for o in out if len(o) == 3], [o for o in out if len(o) == 4]
+    for blocks, threads, chunks in launches:
+        assert blocks == chunks and 0 < blocks * threads < 1 << 32
+    at = {}
+    for i, begin, elements, moved in parts:
+        assert moved and begin == at.get(i, 0) and begin % 2048 == 0 and elements > 0
+        at[i] = begin + elements
+    assert at == {i: n for i, n in enumerate(sizes) if n}
+    if sum(sizes) < 1 << 30:
+        assert len(launches) == -(-sum(n > 0 for n in sizes) // (92 if bits == 8 else 126))
