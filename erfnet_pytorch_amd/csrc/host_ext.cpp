@@ -345,6 +345,20 @@ bool usable(const at::Tensor &t, const char *what)
     return true;
 }
 
+// Stretches of GPU memory (addresses are unique over the devices).
+struct Spans {
+    std::vector<std::pair<const char *, size_t>> of;
+    explicit Spans(size_t most) { of.reserve(most); }
+    void add(const void *p, size_t bytes) { of.emplace_back((const char *)p, bytes); }
+    bool overlap()
+    {
+        if (!std::is_sorted(of.begin(), of.end())) std::sort(of.begin(), of.end());
+        for (size_t i = 1; i < of.size(); ++i)
+            if (of[i - 1].first + of[i - 1].second > of[i].first) return true;
+        return false;
+    }
+};
+
 // A dict read in its own order, which is the order of the questions as a rule, and looked up where it is not.
 struct Walk {
     PyObject *dict, *key = nullptr, *value = nullptr;
@@ -391,6 +405,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     THPObjectPtr missing(PyList_New(0));
     if (!missing) return nullptr;
     std::vector<Batch> batches;
+    Spans spans((size_t)PyList_GET_SIZE(params));
     Walk states(state);
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); ++i) {
         PyObject *obj = PyList_GET_ITEM(params, i);
@@ -418,6 +433,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
             PyErr_Format(PyExc_ValueError, "%sa gradient does not match its parameter", kWho);
             return nullptr;
         }
+        if (n) spans.add(p.const_data_ptr(), p.nbytes());
         if (!st) {
             st = states.find(obj);
             if (!st && PyErr_Occurred()) return nullptr;
@@ -477,6 +493,11 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         b->counts.push_back(count_ptr);
         b->changed.push_back(p.unsafeGetTensorImpl());
     }
+    // (at every step: memory moves with .data, .to() and state dicts behind the optimiser's back)
+    if (spans.overlap()) {
+        PyErr_SetString(PyExc_ValueError, "AdamW: two parameters of one group share memory; their updates would race");
+        return nullptr;
+    }
     if (PyList_GET_SIZE(missing.get())) return missing.release();
     for (const Batch &b : batches) {
         const c10::DeviceGuard guard(b.device);
@@ -496,7 +517,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     END_HANDLE_TH_ERRORS
 }
 
-// share_memory(list of tensors) -> whether two GPU tensors of it overlap (addresses are unique over the devices)
+// share_memory(list of tensors) -> whether two GPU tensors of it overlap
 PyObject *share_memory(PyObject *, PyObject *list)
 {
     HANDLE_TH_ERRORS
@@ -504,18 +525,14 @@ PyObject *share_memory(PyObject *, PyObject *list)
         PyErr_SetString(PyExc_TypeError, "share_memory: (list)");
         return nullptr;
     }
-    std::vector<std::pair<const char *, size_t>> spans;
-    spans.reserve((size_t)PyList_GET_SIZE(list));
+    Spans spans((size_t)PyList_GET_SIZE(list));
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
         PyObject *o = PyList_GET_ITEM(list, i);
         if (!THPVariable_Check(o)) continue;
         const Tensor &t = THPVariable_Unpack(o);
-        if (t.is_cuda() && t.numel()) spans.emplace_back((const char *)t.const_data_ptr(), t.nbytes());
+        if (t.is_cuda() && t.numel()) spans.add(t.const_data_ptr(), t.nbytes());
     }
-    std::sort(spans.begin(), spans.end());
-    for (size_t i = 1; i < spans.size(); ++i)
-        if (spans[i - 1].first + spans[i - 1].second > spans[i].first) Py_RETURN_TRUE;
-    Py_RETURN_FALSE;
+    return PyBool_FromLong(spans.overlap());
     END_HANDLE_TH_ERRORS
 }
 

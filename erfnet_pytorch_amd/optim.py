@@ -244,8 +244,6 @@ class AdamW(torch.optim.Optimizer):
                     float(group["eps"]), float(group["weight_decay"]))
             first = host.adamw_step(*args)
             if first:                   # parameters that have their first gradient: nothing has been launched yet
-                if host.share_memory(group["params"]):       # (they may have come to the GPU after the optimiser was made)
-                    raise ValueError("AdamW: two parameters of one group share memory; their updates would race")
                 with torch.no_grad():
                     for p in first:
                         self.state[p].update(self._new_state(p))

@@ -234,3 +234,37 @@ def test_log_probs_of_more_rows_than_a_launch_of_backward_holds():
     dx, = torch.autograd.grad((r.log_prob, r.entropy), x, (g.repeat(times), g.repeat(times)))
     for part in dx.view(times, tile, v).split(256):
         assert bool((part == dp).all())
+
+
+# ================================================================================ AdamW
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_refuses_parameters_that_come_to_share_memory_later(bits):
+    """Host parameters that come to the GPU on top of each other and have their state from a state dict; parameters that have
+    stepped apart and are moved together.  Nothing is updated, counts included."""
+    from erfnet_pytorch_amd import optim
+
+    def pair(device):
+        return [torch.nn.Parameter(torch.zeros(6, device=device)) for _ in range(2)]
+
+    donor = pair(DEV)
+    first = optim.AdamW(donor, state_bits=bits)
+    for p in donor:
+        p.grad = torch.ones_like(p)
+    first.step()
+    buf = torch.zeros(9, device=DEV)
+    late = pair("cpu")
+    opt = optim.AdamW(late, state_bits=bits)
+    late[0].data, late[1].data = buf[:6], buf[3:]
+    opt.load_state_dict(first.state_dict())
+    for p in late:
+        p.grad = torch.ones(6, device=DEV)
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step()
+    assert not buf.any() and all(float(opt.state[p]["step"]) == 1 for p in late)
+    donor[1].data = donor[0].data
+    with pytest.raises(ValueError, match="share memory"):
+        first.step()
+    donor[1].data = torch.zeros(6, device=DEV)
+    first.step()
+    assert all(float(first.state[p]["step"]) == 2 for p in donor)
