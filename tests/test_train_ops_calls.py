@@ -268,3 +268,47 @@ def test_adamw_refuses_parameters_that_come_to_share_memory_later(bits):
     donor[1].data = torch.zeros(6, device=DEV)
     first.step()
     assert all(float(first.state[p]["step"]) == 2 for p in donor)
+
+
+# ================================================================================ threads
+@gpu
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("op,entry", [("layer_norm", "erf_layer_norm_forward"), ("log_probs", "erf_log_probs_forward")])
+def test_other_python_threads_run_while_a_call_waits(tmp_path, op, entry, grad):
+    """The entry point is exchanged for one that sleeps, as a launch does whose queue is full."""
+    import ctypes
+    import subprocess
+    import threading
+    import time
+    from erfnet_pytorch_amd import _lib, functional as hipf
+    (tmp_path / "nap.c").write_text("#include <unistd.h>\nint nap(void) { usleep(500000); return 0; }\n")
+    subprocess.run(["gcc", "-shared", "-fPIC", "nap.c", "-o", "nap.so"], cwd=tmp_path, check=True, timeout=60)
+    nap = ctypes.CDLL(str(tmp_path / "nap.so")).nap
+    x, target = noise(4, 16).to(DEV).requires_grad_(grad), torch.zeros(4, dtype=torch.int64, device=DEV)
+    host, lib = _lib.host(), _lib.lib()
+
+    def bind(other):
+        host.bind(lambda name: ctypes.cast(other.get(name) or getattr(lib, name), ctypes.c_void_p).value)
+
+    turns, done = [], threading.Event()
+
+    def other():
+        while not done.is_set():
+            turns.append(time.monotonic())
+            time.sleep(0.002)
+
+    thread = threading.Thread(target=other)
+    bind({entry: nap})
+    try:
+        thread.start()
+        begin = time.monotonic()
+        hipf.layer_norm(x) if op == "layer_norm" else hipf.log_probs(x, target)
+        end = time.monotonic()
+    finally:
+        bind({})
+        done.set()
+        thread.join()
+    assert end - begin > 0.4
+    assert sum(begin + 0.05 < t < end - 0.05 for t in turns) > 20
+    y = hipf.layer_norm(x.detach())
+    assert float(y.mean(1).abs().max()) < 1e-6
