@@ -67,18 +67,28 @@ def _run(cmd, verbose):
     subprocess.check_call(cmd)
 
 
+def _host_built_for():
+    """The torch version that _host.so was compiled against (None: no such file, or it does not say)."""
+    if not os.path.exists(_HOST_SO):
+        return None
+    with open(_HOST_SO, "rb") as f:
+        _, found, rest = f.read().partition(b"erfnet_pytorch_amd._host for torch ")
+    return rest[:rest.index(b"\0")].decode() if found else None
+
+
 def build(force=False, verbose=False):
     """Compile csrc/*.hip -> liberfnet_hip.so for gfx950, and csrc/host_ext.cpp -> _host.so (the host side of short
-    calls, against torch's C++ headers), whichever is missing or stale."""
+    calls, against torch's C++ headers), whichever is missing or stale (_host.so also where it was built for another torch)."""
     header = os.path.join(os.path.dirname(_HERE), "include", "erfnet_hip.h")
-    if force or not os.path.exists(_HOST_SO) or \
+    if force or _host_built_for() != torch.__version__ or \
             os.path.getmtime(_HOST_SO) < max(os.path.getmtime(_HOST_SRC), os.path.getmtime(header)):
         base = os.path.dirname(torch.__file__)
         inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"], os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")]
         lib_dir = os.path.join(base, "lib")
         _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", *("-I" + i for i in inc),
-              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__", _HOST_SRC, "-o", _HOST_SO, "-L" + lib_dir,
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__",
+              f'-DERF_TORCH_VERSION="{torch.__version__}"', _HOST_SRC, "-o", _HOST_SO, "-L" + lib_dir,
               "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-Wl,-rpath," + lib_dir], verbose)
     srcs = sources()
     if not force and os.path.exists(_SO) and \
@@ -95,6 +105,10 @@ def host():
     global _host_module
     if _host_module is None:
         handle = lib()
+        made = _host_built_for()
+        if os.path.exists(_HOST_SO) and made != torch.__version__:
+            raise RuntimeError(f"{_HOST_SO} was built for torch {made or '(it does not say)'}, this is {torch.__version__}; build it with "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`")
         try:
             module = importlib.import_module(__package__ + "._host")
         except ImportError as e:

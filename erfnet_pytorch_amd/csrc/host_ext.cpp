@@ -577,6 +577,9 @@ PyObject *bind(PyObject *, PyObject *of)
     END_HANDLE_TH_ERRORS
 }
 
+// Which torch this file was compiled against: _lib.py looks for it in the file before it loads it.
+__attribute__((used)) const char kBuiltFor[] = "erfnet_pytorch_amd._host for torch " ERF_TORCH_VERSION;
+
 PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr},
                          {"layer_norm", (PyCFunction)(void (*)(void))layer_norm, METH_FASTCALL, nullptr},
                          {"log_probs", (PyCFunction)(void (*)(void))log_probs, METH_FASTCALL, nullptr},
