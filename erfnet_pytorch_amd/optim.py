@@ -212,18 +212,32 @@ class AdamW(torch.optim.Optimizer):
                       torch.zeros_like(p, dtype=torch.float8_e4m3fn) for k in self._moments}
 
     def load_state_dict(self, state_dict):
+        # The caller's own hooks belong to it: what the last one before hands on is what is loaded, and the first one after sees
+        # the state as it stays.
+        given = {}
+        before = self.register_load_state_dict_pre_hook(lambda _, final: given.update(self._checked(final)))
+        after = self.register_load_state_dict_post_hook(lambda _: self._restore(given), prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            before.remove()
+            after.remove()
+
+    def _checked(self, state_dict):
         want = set(self._moments)
         for st in state_dict["state"].values():
             if set(st) - {"step"} != want:
                 raise ValueError(f"AdamW(state_bits={self.state_bits}): the state dict holds {sorted(st)}, not "
                                  f"step and {sorted(want)}")
-        super().load_state_dict(state_dict)
+        return state_dict
+
+    def _restore(self, state_dict):
         # torch casts floating-point state to the parameter's type; the moments keep their own
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             if i in state_dict["state"]:
                 given = state_dict["state"][i]
-                for k in want:
+                for k in self._moments:
                     # (torch.optim.AdamW keeps a bf16 parameter's moments in bf16)
                     dtype = given[k].dtype if given[k].dtype == torch.float8_e4m3fn else torch.float32
                     self.state[p][k] = given[k].detach().to(p.device, dtype, copy=True).contiguous()

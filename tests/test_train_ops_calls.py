@@ -270,6 +270,44 @@ def test_adamw_refuses_parameters_that_come_to_share_memory_later(bits):
     assert all(float(first.state[p]["step"]) == 2 for p in donor)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_load_state_dict_minds_the_callers_hooks(bits):
+    """(CPU.)  A hook before hands on another dict: that one is loaded.  A hook after sees the state as it stays, with the moments'
+    own types, and what it does to it stays."""
+    from erfnet_pytorch_amd import optim
+    p = torch.nn.Parameter(noise(300, dtype=torch.bfloat16))
+    opt = optim.AdamW([p], state_bits=bits)
+    state = opt._new_state(p)
+    key = opt._moments[0]
+    saved = opt.state_dict()
+    saved["state"] = {0: {**state, "step": torch.tensor(3.0)}}
+
+    def before(optimizer, given):
+        entry = given["state"][0]
+        return {**given, "state": {0: {**entry, "step": entry["step"] + 4, key: torch.ones_like(entry[key], dtype=torch.float32).to(
+            entry[key].dtype)}}}
+
+    seen = []
+
+    def after(optimizer):
+        entry = optimizer.state[p]
+        seen.append({k: v.dtype for k, v in entry.items()})
+        entry["step"] += 10
+
+    opt.register_load_state_dict_pre_hook(before)
+    opt.register_load_state_dict_post_hook(after)
+    for turn in (1, 2):
+        opt.load_state_dict(saved)
+        assert len(seen) == turn and seen[-1] == {k: v.dtype for k, v in state.items()}
+        assert float(opt.state[p]["step"]) == 17 and bool((opt.state[p][key].float() == 1).all())
+        assert opt.state[p][key].data_ptr() != saved["state"][0][key].data_ptr()
+    bad = {**saved, "state": {0: {"step": torch.tensor(1.0)}}}
+    with pytest.raises((ValueError, KeyError)):
+        opt.load_state_dict(bad)
+    opt.load_state_dict(saved)
+    assert len(seen) == 3
+
+
 # ================================================================================ threads
 @gpu
 @pytest.mark.parametrize("grad", [False, True])
