@@ -180,10 +180,18 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: state_bits must be 8 or 32 (got {state_bits})")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False,
                                       maximize=False, foreach=None, capturable=False, differentiable=False,
-                                      fused=None, decoupled_weight_decay=True))
-        self.defaults["state_bits"] = state_bits        # (what a copied or unpickled optimiser keeps)
+                                      fused=None, decoupled_weight_decay=True, state_bits=state_bits))
 
     def add_param_group(self, param_group):
+        if isinstance(param_group, dict) and not isinstance(param_group["params"], set):      # (torch refuses the others)
+            param_group = self._checked_group(param_group)
+        super().add_param_group(param_group)
+        # the whole optimiser's, kept in its defaults (which a copied or unpickled one has too); groups hold torch's keys
+        self.param_groups[-1].pop("state_bits", None)
+
+    def _checked_group(self, param_group):
+        if param_group.get("state_bits", self.state_bits) != self.state_bits:
+            raise ValueError(f"AdamW: state_bits is one for all groups ({self.state_bits}), not {param_group['state_bits']} for one")
         params = param_group["params"]
         params = [params] if isinstance(params, torch.Tensor) else list(params)
         tensors = [p[1] if isinstance(p, tuple) else p for p in params]
@@ -191,7 +199,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: a parameter appears twice in one group; its two updates would race")
         if any(getattr(p, "is_cuda", False) for p in tensors) and _lib.host().share_memory(tensors):
             raise ValueError("AdamW: two parameters of one group share memory; their updates would race")
-        super().add_param_group({**param_group, "params": params})
+        return {**param_group, "params": params}
 
     @property
     def state_bits(self):

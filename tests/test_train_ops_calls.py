@@ -308,6 +308,30 @@ def test_adamw_load_state_dict_minds_the_callers_hooks(bits):
     assert len(seen) == 3
 
 
+def test_adamw_groups_are_refused_as_torch_refuses_them_and_hold_its_keys():
+    """(CPU.)  A set has no order to put the state in; state_bits is the optimiser's, and was ignored where a group gave another."""
+    import copy
+    import pickle
+    from erfnet_pytorch_amd import optim
+    a, b, c = (torch.nn.Parameter(torch.zeros(3)) for _ in range(3))
+    opt = optim.AdamW([a], state_bits=8)
+    with pytest.raises(TypeError, match="ordered"):
+        opt.add_param_group({"params": {b}})
+    with pytest.raises(TypeError, match="dict"):
+        opt.add_param_group([b])
+    with pytest.raises(ValueError, match="state_bits"):
+        opt.add_param_group({"params": [b], "state_bits": 32})
+    with pytest.raises(ValueError, match="state_bits"):
+        optim.AdamW([{"params": [a], "state_bits": 8}])
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": (p for p in [b]), "state_bits": 8, "lr": 1e-5})
+    opt.add_param_group({"params": c})
+    keys = set(torch.optim.AdamW([torch.nn.Parameter(torch.zeros(3))]).param_groups[0])
+    for o in (opt, copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert o.state_bits == 8 and all(set(g) == keys for g in o.param_groups)
+    assert [g["lr"] for g in opt.param_groups] == [1e-3, 1e-5, 1e-3]
+
+
 # ================================================================================ threads
 @gpu
 @pytest.mark.parametrize("grad", [False, True])
