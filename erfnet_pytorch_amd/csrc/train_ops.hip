@@ -390,7 +390,12 @@ int adamw_step(const char *what, int count, void *const *p, const void *const *g
     d.k.keep = (float)(1.0 - lr * wd);
     d.k.step = (float)(lr / (1.0 - pow(b1, (double)step)));
     d.k.inv_root_c2 = (float)(1.0 / sqrt(1.0 - pow(b2, (double)step)));
-    d.k.eps = (float)eps;
+    // The reciprocal takes a subnormal number for zero, and an element without a gradient so far has eps alone below its line:
+    // the quotient is formed 2^24 fold above and below then (roots are under 2^64, so nothing overflows).
+    const double least = 1.1754943508222875e-38, fold = eps > 0.0 && eps < least ? 16777216.0 : 1.0;
+    d.k.eps = fold == 1.0 ? (float)eps : (float)std::max(eps * fold, least);
+    d.k.inv_root_c2 *= (float)fold;
+    d.k.step *= (float)fold;
     long long elements = 0;
     for (int i = 0; i < count; ++i) {
         if (numel[i] < 0) return fail("%s: tensor %d has a negative size", what, i);

@@ -332,6 +332,22 @@ def test_adamw_groups_are_refused_as_torch_refuses_them_and_hold_its_keys():
     assert [g["lr"] for g in opt.param_groups] == [1e-3, 1e-5, 1e-3]
 
 
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [2.0 ** -126, 1e-40, 2.0 ** -149, 1e-300])
+def test_adamw_with_an_eps_below_the_normal_numbers(eps, bits):
+    """No gradient so far: 0 / (0 + eps) = 0, however small eps is."""
+    from erfnet_pytorch_amd import optim
+    p = torch.nn.Parameter(noise(300).to(DEV))
+    was = p.detach().clone()
+    p.grad = torch.zeros_like(p)
+    p.grad[::2] = 1.0
+    optim.AdamW([p], lr=1e-2, eps=eps, weight_decay=0.0, state_bits=bits).step()
+    assert torch.equal(p[1::2], was[1::2])
+    # lr m / c1 / sqrt(v / c2) = lr: root, reciprocal and scalars to a few units each, and the difference's own rounding
+    assert float((was[::2] - p.detach()[::2] - 1e-2).abs().max()) <= 32 * 2.0 ** -24 * 1e-2 + 2.0 ** -24 * 4
+
+
 # ================================================================================ threads
 @gpu
 @pytest.mark.parametrize("grad", [False, True])
