@@ -6,6 +6,7 @@ shape stays [N,C,H,W], i.e. ``torch.channels_last``); the classifier logits leav
 transposed convolution NCHW-contiguous so that torch's loss / argmax read them directly.
 """
 import ctypes as C
+import operator
 import os
 from typing import NamedTuple
 
@@ -1341,8 +1342,9 @@ def log_probs(logits, target, top_k=0, dim=-1, ignore_index=-1):
         raise ValueError(f"log_probs: target shape {tuple(target.shape)} does not match logits {shape} without dim {dim}")
     if not 1 <= v <= 1 << 30:
         raise ValueError(f"log_probs: 1..{1 << 30} classes (got {v})")
+    top_k, ignore_index = operator.index(top_k), operator.index(ignore_index)
     if not 0 <= top_k <= min(64, v):
         raise ValueError(f"log_probs: top_k must be in 0..{min(64, v)} (got {top_k})")
     _need_gpu("log_probs", logits, target)
     _materialize_logits(logits)
-    return LogProbs(*_lib.host().log_probs(logits, target, int(top_k), int(ignore_index), axis))
+    return LogProbs(*_lib.host().log_probs(logits, target, top_k, ignore_index, axis))

@@ -213,6 +213,17 @@ def test_layer_norm_error_goes_with_the_spread_and_not_with_the_level(c):
     assert float(((y - ref).abs() / bound).max()) <= 1
 
 
+def test_log_probs_takes_whole_numbers():
+    """(CPU: decided before the tensors are looked at.)  2.5 was taken for 2."""
+    from erfnet_pytorch_amd import functional as hipf
+    x, target = noise(4, 16), torch.zeros(4, dtype=torch.int64)
+    for bad in (dict(top_k=2.5), dict(top_k=2.0), dict(top_k=2, ignore_index=0.5)):
+        with pytest.raises(TypeError):
+            hipf.log_probs(x, target, **bad)
+    with pytest.raises(RuntimeError, match="cpu"):
+        hipf.log_probs(x, target, top_k=torch.tensor(2), ignore_index=torch.tensor(-1))
+
+
 # ================================================================================ sizes
 @gpu
 def test_log_probs_of_more_rows_than_a_launch_of_backward_holds():
