@@ -401,3 +401,27 @@ def test_other_python_threads_run_while_a_call_waits(tmp_path, op, entry, grad):
     assert sum(begin + 0.05 < t < end - 0.05 for t in turns) > 20
     y = hipf.layer_norm(x.detach())
     assert float(y.mean(1).abs().max()) < 1e-6
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,v", [(1301, 20011), (40_001, 701)])
+def test_every_entry_of_a_streamed_gradient_equals_that_of_small_calls(rows, v, kind):
+    """Gradients of 48 MB and more are stored past the caches, those of 576 rows are not.  576 rows begin at the same place of a
+    cache line in both, and a row has the same threads at either count, so every entry is the same bit for bit."""
+    from erfnet_pytorch_amd import functional as hipf
+    g = torch.Generator(device=DEV).manual_seed(v)
+    x = torch.randn(rows, v, generator=g, device=DEV).to(kind)
+    t = torch.randint(0, v, (rows,), generator=g, device=DEV)
+    ups = [torch.randn(rows, generator=g, device=DEV), torch.randn(rows, generator=g, device=DEV),
+           torch.randn(rows, 3, generator=g, device=DEV)]
+    assert x.nbytes >= 48 << 20 > 576 * v * x.element_size()
+
+    def gradient(a, b):
+        part = x[a:b].clone().requires_grad_()
+        r = hipf.log_probs(part, t[a:b], 3)
+        return torch.autograd.grad([r.log_prob, r.entropy, r.top_log_probs], part, [u[a:b] for u in ups])[0]
+
+    whole = gradient(0, rows)
+    for a in range(0, rows, 576):
+        assert torch.equal(whole[a:a + 576], gradient(a, min(a + 576, rows))), a
