@@ -425,3 +425,56 @@ def test_every_entry_of_a_streamed_gradient_equals_that_of_small_calls(rows, v, 
     whole = gradient(0, rows)
     for a in range(0, rows, 576):
         assert torch.equal(whole[a:a + 576], gradient(a, min(a + 576, rows))), a
+
+
+@gpu
+def test_every_entry_of_gradients_beyond_32_bit_offsets():
+    """The last 288 of 32800 rows of 65537 classes (2^31 elements end within them) beside the same rows by themselves: as many
+    blocks a row and the same place of a cache line, so all of dx is the same bit for bit, the small entries too."""
+    from erfnet_pytorch_amd import functional as hipf
+    v, rows, tail = 65537, 32800, 288
+    g = torch.Generator(device=DEV).manual_seed(1)
+    part = (3 * torch.randn(tail, v, generator=g, device=DEV)).bfloat16()
+    t = torch.randint(0, v, (tail,), generator=g, device=DEV)
+    ups = [torch.randn(tail, generator=g, device=DEV), torch.randn(tail, generator=g, device=DEV),
+           torch.randn(tail, 4, generator=g, device=DEV)]
+    x = torch.zeros(rows, v, dtype=torch.bfloat16, device=DEV)
+    x[-tail:] = part
+    assert (rows - tail) * v < 1 << 31 < rows * v and (rows - tail) * v * 2 % 128 == 0
+
+    def run(x, t, ups):
+        x = x.requires_grad_()
+        r = hipf.log_probs(x, t, 4)
+        return [*(o.detach()[-tail:] for o in r),
+                torch.autograd.grad([r.log_prob, r.entropy, r.top_log_probs], x, ups)[0][-tail:]]
+
+    def padded(u):
+        return torch.cat([u.new_zeros(rows - tail, *u.shape[1:]), u])
+
+    for a, b in zip(run(x, padded(t), [padded(u) for u in ups]), run(part, t, ups)):
+        assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("c", [20, 1000, 5000])
+def test_layer_norm_with_a_variance_below_the_normal_numbers(c, kind):
+    """Equal values and an eps of 1e-40: y = bias, dx = (g - mean g) / sqrt(eps) (eps rounds to 2^-149 in fp32: 1e-5 of itself).
+    Spreads of 2^-66 and no eps: the squares keep 2^-18 of themselves (they are near 2^-132, rounded to 2^-149), the
+    root half of that; the rest is as ever."""
+    from erfnet_pytorch_amd import functional as hipf
+    own, u = (0.0 if kind == torch.float32 else 2.0 ** -8), 2.0 ** -24
+    b = noise(c, seed=1)
+    g = noise(3, c, seed=2, dtype=kind)
+    x = torch.full((3, c), 0.75, dtype=kind).to(DEV).requires_grad_()
+    y = hipf.layer_norm(x, None, b.to(DEV), eps=1e-40)
+    assert torch.equal(y, b.to(DEV).to(kind).expand_as(y))
+    dx, = torch.autograd.grad(y, x, g.to(DEV))
+    mean = g.double().mean(1, keepdim=True)
+    ref, size = (g.double() - mean) * 1e20, (g.double().abs() + g.double().abs().mean(1, keepdim=True)) * 1e20
+    assert float(((dx.cpu().double() - ref).abs() - (2e-5 + 72 * u) * size * (1 + own) - own * ref.abs()).max()) <= 0
+    x = noise(3, c, seed=c, dtype=kind) * 2.0 ** -66
+    y = hipf.layer_norm(x.to(DEV), eps=0.0).cpu().double()
+    d = x.double() - x.double().mean(1, keepdim=True)
+    ref = d / torch.sqrt((d * d).mean(1, keepdim=True))
+    assert float(((y - ref).abs() - (2.0 ** -18 + 72 * u) * (1 + ref.abs()) * (1 + own) - own * ref.abs()).max()) <= 0
