@@ -19,6 +19,7 @@
 #include <torch/csrc/utils/object_ptr.h>
 
 #include <algorithm>
+#include <deque>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -68,7 +69,10 @@ Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const Tensor &beside, b
     return Tensor(at::detail::empty_cuda(shape, type, beside.device(),
                                          image ? at::MemoryFormat::ChannelsLast : at::MemoryFormat::Contiguous));
 }
-Tensor parameter(const Tensor &t) { return t.defined() ? t.to(at::kFloat).contiguous() : t; }
+// The numbers themselves, where t is a view that stands for its negative (the imaginary part of a conjugate; such a view of one
+// number counts as contiguous).
+Tensor numbers(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor parameter(const Tensor &t) { return t.defined() ? numbers(t.to(at::kFloat).contiguous()) : t; }
 
 // What backward returns, from an operator whose gradient has none: where a graph of the backward pass is recorded
 // (`recorded`), the results hang on a node that raises, in front of everything that they depend on: the upstream gradients,
@@ -109,7 +113,7 @@ void no_tracing(const char *what)
 // Rows of C contiguous channels: the last axis as it is, axis 1 of an image as NHWC memory.
 Tensor norm_rows(const Tensor &x, bool image)
 {
-    return image ? x.contiguous(at::MemoryFormat::ChannelsLast) : x.contiguous();
+    return numbers(image ? x.contiguous(at::MemoryFormat::ChannelsLast) : x.contiguous());
 }
 
 Tensor norm_forward(const Tensor &x, const Tensor &w, const Tensor &b, double eps, bool image, Tensor *stat)
@@ -204,6 +208,7 @@ variable_list logp_forward(const Tensor &logits, const Tensor &target0, LogpShap
         if (x.stride(1) != 1 || (pixels > 1 && x.stride(0) < s.v)) x = x.contiguous();
         s.ld = pixels > 1 ? x.stride(0) : s.v;
     }
+    x = numbers(x);
     for (int64_t i = 0; i < nd; ++i)
         if (i != s.axis) full.push_back(logits.size(i));
         else if (!s.moved) full.push_back(s.top_k);
@@ -250,7 +255,7 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
         Tensor g[3];
         for (int i = 0; i < 3; ++i)
             if (grads[i].defined())
-                g[i] = (moved && i == 2 ? grads[i].movedim(axis, -1) : grads[i]).to(at::kFloat).contiguous();
+                g[i] = numbers((moved && i == 2 ? grads[i].movedim(axis, -1) : grads[i]).to(at::kFloat).contiguous());
         if (moved) {
             shape.push_back(shape[axis]);
             shape.erase(shape.begin() + axis);
@@ -351,8 +356,8 @@ bool usable(const at::Tensor &t, const char *what)
                      "tensors)", kWho, what, t.device().str().c_str());
         return false;
     }
-    if (!t.is_contiguous()) {
-        PyErr_Format(PyExc_ValueError, "%s%s is not contiguous", kWho, what);
+    if (!t.is_contiguous() || t.is_neg()) {
+        PyErr_Format(PyExc_ValueError, "%s%s is %s", kWho, what, t.is_neg() ? "a view of its negative" : "not contiguous");
         return false;
     }
     return true;
@@ -420,6 +425,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     THPObjectPtr missing(PyList_New(0));
     if (!missing) return nullptr;
     std::vector<Batch> batches;
+    std::deque<Tensor> resolved;            // gradients that are written for the launch (on its stream, as they are read)
     Spans spans((size_t)PyList_GET_SIZE(params));
     Walk states(state);
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); ++i) {
@@ -430,8 +436,14 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         }
         PyObject *st = states.next_if(obj);
         const at::Tensor &p = THPVariable_Unpack(obj);
-        const at::Tensor &g = p.grad();
-        if (!g.defined()) continue;
+        const at::Tensor *grad = &p.grad();
+        if (!grad->defined()) continue;
+        if (grad->is_neg()) {
+            const at::NoGradGuard no_grad;
+            resolved.push_back(grad->resolve_neg());
+            grad = &resolved.back();
+        }
+        const at::Tensor &g = *grad;
         if (g.is_sparse()) {
             PyErr_Format(PyExc_RuntimeError, "%ssparse gradients are not supported", kWho);
             return nullptr;

@@ -359,6 +359,66 @@ def test_adamw_with_an_eps_below_the_normal_numbers(eps, bits):
     assert float((was[::2] - p.detach()[::2] - 1e-2).abs().max()) <= 32 * 2.0 ** -24 * 1e-2 + 2.0 ** -24 * 4
 
 
+# ================================================================================ views that stand for their negative
+def negative(t):
+    """A contiguous view that stands for t, of memory that holds -t: what autograd leaves as the gradient of a single number that
+    became the imaginary part of a complex one."""
+    view = torch._neg_view(-t)
+    assert view.is_neg() and view.is_contiguous()
+    return view
+
+
+@gpu
+def test_gradient_of_a_number_in_complex_arithmetic_has_its_sign():
+    from erfnet_pytorch_amd import optim
+    p = torch.nn.Parameter(torch.zeros(1, device=DEV))
+    z = torch.complex(torch.zeros(1, device=DEV), p)
+    z.conj().backward(torch.full((1,), 1 + 2j, device=DEV))
+    assert p.grad.is_neg() and float(p.grad) == -2
+    optim.AdamW([p], lr=0.25, weight_decay=0.0).step()
+    assert abs(float(p.detach()) - 0.25) < 1e-6
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_with_negated_views(bits):
+    from erfnet_pytorch_amd import optim
+    init, grad, new = noise(700, seed=1), noise(700, seed=2), []
+    for wrap in (torch.clone, negative):
+        p = torch.nn.Parameter(init.to(DEV))
+        opt = optim.AdamW([p], state_bits=bits)
+        for _ in range(2):
+            p.grad = wrap(grad.to(DEV))
+            opt.step()
+        new.append(p.detach())
+    assert torch.equal(*new)
+    q = torch.nn.Parameter(negative(init.to(DEV)))
+    q.grad = grad.to(DEV)
+    if q.is_neg():
+        with pytest.raises(ValueError, match="negative"):
+            optim.AdamW([q], state_bits=bits).step()
+
+
+@gpu
+def test_layer_norm_and_log_probs_of_negated_views():
+    from erfnet_pytorch_amd import functional as hipf
+    t = {n: noise(*s, seed=i).to(DEV) for i, (n, s) in enumerate(
+        dict(x=(4, 16), w=(16,), b=(16,), gy=(4, 16), image=(2, 8, 3, 5), logits=(4, 40), pixels=(2, 8, 3, 5), g=(4,), gp=(2, 3, 5)).items())}
+    rows, map_ = torch.arange(4, device=DEV), torch.ones(2, 3, 5, dtype=torch.int64, device=DEV)
+
+    def work(wrap):
+        v = {n: wrap(a).requires_grad_() for n, a in t.items()}
+        y = hipf.layer_norm(v["x"], v["w"], v["b"])
+        out = [y, *torch.autograd.grad(y, (v["x"], v["w"], v["b"]), v["gy"].detach()), hipf.layer_norm(v["image"], dim=1)]
+        for x, target, dim, g in ((v["logits"], rows, -1, v["g"]), (v["pixels"], map_, 1, v["gp"])):
+            r = hipf.log_probs(x, target, top_k=2, dim=dim)
+            out += [*r, *torch.autograd.grad((r.log_prob, r.entropy), x, (g.detach(), g.detach()))]
+        return out
+
+    for a, b in zip(work(torch.clone), work(negative)):
+        assert torch.equal(a, b)
+
+
 # ================================================================================ threads
 @gpu
 @pytest.mark.parametrize("grad", [False, True])
