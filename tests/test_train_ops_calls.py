@@ -538,3 +538,38 @@ def test_layer_norm_with_a_variance_below_the_normal_numbers(c, kind):
     d = x.double() - x.double().mean(1, keepdim=True)
     ref = d / torch.sqrt((d * d).mean(1, keepdim=True))
     assert float(((y - ref).abs() - (2.0 ** -18 + 72 * u) * (1 + ref.abs()) * (1 + own) - own * ref.abs()).max()) <= 0
+
+
+@gpu
+def test_two_threads_call_at_once_on_streams_of_their_own():
+    import threading
+    from erfnet_pytorch_amd import functional as hipf, optim
+    target = torch.arange(9, device=DEV)
+
+    def work(seed):
+        x, w = noise(9, 3000, seed=seed).to(DEV), torch.nn.Parameter(1 + 0.1 * noise(3000, seed=seed + 1).to(DEV))
+        opt = optim.AdamW([w], lr=1e-2, state_bits=8 if seed % 2 else 32)
+        for _ in range(20):
+            w.grad = None
+            r = hipf.log_probs(hipf.layer_norm(x, w), target, 4)
+            (r.log_prob.sum() + r.entropy.sum() + r.top_log_probs.sum()).backward()
+            opt.step()
+        return w.detach()
+
+    alone = [work(s) for s in (1, 2)]
+    got = [None, None]
+
+    def thread(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[i] = work(i + 1)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    torch.cuda.synchronize()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(alone, got):
+        assert torch.equal(a, b)
