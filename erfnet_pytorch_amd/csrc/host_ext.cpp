@@ -1,7 +1,7 @@
 // erfnet_pytorch_amd._host: the host side of the calls that are shorter than their Python would be.
 //   layer_norm, log_probs: autograd nodes over the C ABI (with a backward pass that enters Python from autograd's
 //     thread, log probabilities of 256 x 1000 with gradients took 117 us around 15 us of kernels; 67 so);
-//   adamw_step: one pass over the parameters (229 of them, 20 us of GPU work: 583 us a step in Python, 31 so).
+//   adamw_step: one pass over the parameters (229 of them, 20 us of GPU work: 583 us a step in Python, 33 so).
 // Arguments come checked from functional.py / optim.py.  Nothing is kept between calls.
 #include <Python.h>
 

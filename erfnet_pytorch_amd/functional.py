@@ -1288,7 +1288,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, dim=-1):
     """(x - mean) / sqrt(var + eps) * weight + bias over one axis, with its gradients: the last axis, or ``dim=1`` of an
     [N,C,H,W] activation (every pixel over its channels, which are contiguous in the framework's NHWC memory).  x fp32 or
     bf16 with 1..16384 channels; weight, bias: [C] or None.  The result has x's type; statistics, products and sums are
-    fp32.  No counterpart in the reference, whose blocks normalise over the batch (train/erfnet_blocks.py:23)."""
+    fp32.  Second derivatives, forward mode and tracing raise.  No counterpart in the reference, whose blocks normalise over
+    the batch (train/erfnet_blocks.py:23)."""
     _check_act(x)
     nd = x.dim()
     axis = dim + nd if dim < 0 else dim
@@ -1327,7 +1328,7 @@ def log_probs(logits, target, top_k=0, dim=-1, ignore_index=-1):
     has log probabilities of -infinity, entropy 0 and no gradient.  A NaN or +infinity makes its row NaN.
 
     Rows of contiguous classes (the last axis, also with a stride between rows) and pixels ([N,K,H,W], dim 1) are read in
-    place; other layouts are copied into rows first.  The reference has only the mean of the first result
+    place; other layouts are copied into rows first.  Second derivatives, forward mode and tracing raise.  The reference has only the mean of the first result
     (CrossEntropyLoss2d, train/evaluation_functions.py:6-14)."""
     _check_act(logits)
     nd = logits.dim()

@@ -169,7 +169,8 @@ class AdamW(torch.optim.Optimizer):
     that holds several parameters (``ddp.GradientReducer.flatten_parameters``) the 256 elements of a scale run across them:
     fp32 moments give the update of the separate tensors bit for bit, 8-bit ones to their rounding.
 
-    ``step`` cannot be captured into a HIP graph (the library refuses): the bias corrections go into the launch."""
+    ``step`` cannot be captured into a HIP graph (the library refuses): the bias corrections go into the launch.  Parameters of
+    a group whose memory overlaps are refused, at every step: their updates run side by side."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
         if lr < 0.0 or eps < 0.0 or weight_decay < 0.0:
