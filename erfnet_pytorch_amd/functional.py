@@ -1328,8 +1328,8 @@ def log_probs(logits, target, top_k=0, dim=-1, ignore_index=-1):
     has log probabilities of -infinity, entropy 0 and no gradient.  A NaN or +infinity makes its row NaN.
 
     Rows of contiguous classes (the last axis, also with a stride between rows) and pixels ([N,K,H,W], dim 1) are read in
-    place; other layouts are copied into rows first.  Second derivatives, forward mode and tracing raise.  The reference has only the mean of the first result
-    (CrossEntropyLoss2d, train/evaluation_functions.py:6-14)."""
+    place; other layouts are copied into rows first.  Second derivatives, forward mode and tracing raise.  The reference has
+    only the mean of the first result (CrossEntropyLoss2d, train/evaluation_functions.py:6-14)."""
     _check_act(logits)
     nd = logits.dim()
     if nd < 1 or not -nd <= dim < nd:
